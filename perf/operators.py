@@ -60,7 +60,7 @@ def draw(rng):
         m = _size(rng, 1, max(1, min(8192, MOST_MACS // (batch * n * k))))
         a = rng.choice(["int8", "int8", "fp8_143", "fp8_152"])
         b = "int8" if a == "int8" else rng.choice(["fp8_143", "fp8_152"])
-        out = rng.choice(["bf16", "bf16", "fp16", "fp32"] + (["int32"] if a == "int8" else []))
+        out = rng.choice(["bf16", "bf16", "fp16"] + (["fp32", "int32"] if a == "int8" else []))
         return {"op": op, "batch": batch, "m": m, "n": n, "k": k, "a": a, "b": b, "out": out, "bias": out != "int32" and rng.random() < 0.5}
     width = _size(rng, 64, 16384, rng.choice([1, 8, 64]))
     case = {"op": op, "rows": _size(rng, 1, min(16384, MOST_CELLS // width)), "width": width, "type": rng.choice(["bf16", "bf16", "fp16", "fp32"]),
