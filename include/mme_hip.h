@@ -70,6 +70,21 @@ enum
     MME_HIP_UFP16 = 17 /* unsigned fp16, 0-6-10, configurable exponent bias (default 31); e_types_nr is 16 */
 };
 
+/* Element types of the 8-bit linear layer (mme_hip_quantize_rows_dev, mme_hip_rms_norm_quantize_dev, mme_hip_scaled_gemm_dev) that
+ * the other entry points do not take.  The numbers are this library's own, behind those of the reference's enum. */
+enum
+{
+    MME_HIP_INT8 = 32, /* two's complement; the quantisers write -127 .. 127, the product takes every code */
+    MME_HIP_INT32 = 33 /* the sums of a product of int8 codes */
+};
+
+/* gate of mme_hip_quantize_rows_dev */
+enum
+{
+    MME_HIP_GATE_SILU = 0,     /* g / (1 + e^-g)                                               */
+    MME_HIP_GATE_GELU_TANH = 1 /* g / 2 (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3)))            */
+};
+
 /* MmeCommon::RoundingMode (mme_common_enum.h:65-80). */
 enum
 {
@@ -505,6 +520,91 @@ int mme_hip_cast_to_fp32_dev(mme_hip_handle h,
  * reference's harness computes it on the host (no reference function).
  */
 int mme_hip_absmax_dev(mme_hip_handle h, float* out_absmax, const float* in, size_t n);
+
+/* ---- 8-bit linear layer: row quantisers and the scaled product ------------- */
+
+/*
+ * A linear layer in 8 bits with a scale per token and per output channel (no counterpart in the reference, whose scales are
+ * exponent biases and powers of two): the quantisers turn rows of values into rows of codes and one fp32 scale each, the product
+ * multiplies codes by codes and applies the scales.  All three take device pointers, enqueue one kernel (the product two where
+ * it splits a reduction) on the handle's stream, whichever device is current, and can be recorded into a graph.
+ *
+ * A row is dimension 0 of a tensor (sizes[0] elements, contiguous); dimensions 1 .. 4 enumerate rows, with any strides.
+ * Input rows may share memory (stride 0: the same row for every index); output rows may not, and an output's memory
+ * (first to last element) must not meet an input's, the one exception being named below: EINVAL.  Only the elements of a tensor
+ * are read and written, whatever lies between or behind its rows.  Pointers are aligned to their element type, no further.
+ *
+ * mme_hip_quantize_rows_dev:  v = x, or v = gate(g) x when `gate` is not NULL (a gated feed-forward block's input of its second
+ * projection), then for every row
+ *     scale = max |v| / q,   code_i = v_i / scale rounded to nearest even,   v_i ~ code_i scale
+ * with q the largest value of the output type: 127 (MME_HIP_INT8); 240 2^(7-bias) (fp8_143 in full inf/NaN mode) or 448 2^(7-bias)
+ * (minimal mode); 57344 2^(15-bias) (fp8_152 in full mode).  Other inf/NaN modes: EUNSUPPORTED.  No code is an inf or NaN.
+ * x and gate: bf16, fp16 (exponent bias 15, full mode) or fp32, the same type and sizes as each other; the sizes of out.
+ * row_scales: one float per row, dense in the order of the rows (dimension 1 fastest).  Arithmetic in fp32, the scale is
+ * rounded once from fp64.  A row of zeros gets the scale 0 and codes of zero.  A row that holds an inf or NaN (or whose gated
+ * products overflow fp32) gets the scale NaN and codes 0: NaN reaches every output of its row in the product, and no other.
+ * Where the scale itself falls below 2^-126 it has fewer bits, like any denormal.
+ */
+int mme_hip_quantize_rows_dev(mme_hip_handle        h,
+                              const mme_hip_tensor* out,
+                              float*                row_scales,
+                              const mme_hip_tensor* x,
+                              const mme_hip_tensor* gate, /* may be NULL */
+                              int                   gate_op);
+
+/*
+ * Root-mean-square norm with the residual's addition, quantised like that:
+ *     s = x + residual (fp32),   residual_out = s rounded to x's type,   v_i = s_i gamma_i / sqrt(mean(s^2) + eps)
+ * The norm works on s before it is rounded.  residual and residual_out (types and sizes of x) may be NULL: s = x, and the sum is
+ * not kept; residual_out needs a residual and may be x or residual themselves (the same descriptor: in place).  gamma: sizes[0]
+ * elements in one row, of x's type or fp32, NULL for ones.  eps: finite, >= 0.  A row whose s or s gamma holds an inf or NaN
+ * has the scale NaN and codes 0 (residual_out is written as it is); finite values of any size are normalised without
+ * overflow.  A row of zeros has the scale 0, also with eps 0.
+ */
+int mme_hip_rms_norm_quantize_dev(mme_hip_handle        h,
+                                  const mme_hip_tensor* out,
+                                  float*                row_scales,
+                                  const mme_hip_tensor* residual_out, /* may be NULL */
+                                  const mme_hip_tensor* x,
+                                  const mme_hip_tensor* residual,     /* may be NULL */
+                                  const mme_hip_tensor* gamma,        /* may be NULL */
+                                  float                 eps);
+
+/*
+ * out[m][n] = (sum over k of x[m][k] w[n][k]) x_scales[m] w_scales[n] + bias[n]
+ * (the "abt" form of mme_hip_batch_gemm_dev: x is [K, M, batch], w [K, N, batch], out [N, M, batch]; a batch dimension of size 1
+ * of an operand broadcasts, and its scales with it).  x_scales: one float per row of x, w_scales and bias: one per row of w,
+ * dense in the order of the operand's rows; each may be NULL (ones, ones, zeros).
+ *   int8 x int8: sums in int32, exact; K <= 131071 (no sum of that length can overflow; longer: EUNSUPPORTED).  out: bf16,
+ *     fp16, fp32, or MME_HIP_INT32: the sums, x_scales, w_scales and bias NULL.
+ *   fp8 x fp8 (either flavour each, any exponent bias mme_hip_batch_gemm_dev takes): sums in fp32, formed by the matrix cores: of
+ *     every eight products of consecutive k, what lies below 2^-13 of the largest one's power of two is dropped before they are
+ *     added (about 5e-5 of a sum of random codes).  out: bf16, fp16; fp32 outputs, which would promise more than these
+ *     sums hold: EUNSUPPORTED.  The operands are read as the hardware's e4m3 / e5m2, which is what fp8_143 in minimal and fp8_152
+ *     in full inf/NaN mode mean; other modes need the promise MME_HIP_FP8_SPECIALS_ASSUME_NONE (mme_hip_set_fp8_specials_policy) that no
+ *     code has all exponent bits set, which holds for what the quantisers write: EUNSUPPORTED without it.
+ * The sum is rounded to fp32, multiplied by the scale of x, then by that of w (together with the addition of the bias in one
+ * rounding), then rounded to nearest even into out's type; out of range becomes inf.  fp16 outputs have exponent bias 15.
+ * The result does not depend on which rows are computed together nor on timing: it is the same for every call with the same operands and
+ * sizes.  K = 0 gives the bias.  Up to 65535 batch elements.
+ * With a split reduction the partial sums go to a work space of the handle (see mme_hip_set_stream; for recording, see
+ * mme_hip_batch_gemm_dev_noalloc: call once with these sizes before the recording starts).
+ */
+int mme_hip_scaled_gemm_dev(mme_hip_handle        h,
+                            const mme_hip_tensor* out,
+                            const mme_hip_tensor* x,
+                            const float*          x_scales, /* may be NULL */
+                            const mme_hip_tensor* w,
+                            const float*          w_scales, /* may be NULL */
+                            const float*          bias);    /* may be NULL */
+
+/*
+ * What mme_hip_scaled_gemm_dev would launch for these descriptors, like mme_hip_plan_batch_gemm: form[0] 0 the general kernel, 1 a
+ * tile kernel, 3 the kernel for few rows of x; form[1] rows of x per workgroup; form[2] slices of the reduction; form[3] wavefronts
+ * per workgroup.  mme_hip_last_contraction_form reports the same after a call.
+ */
+int mme_hip_plan_scaled_gemm(const mme_hip_tensor* out, const mme_hip_tensor* x, const mme_hip_tensor* w, int num_cus, int fp8_specials_policy,
+                             int form[4], char* error, size_t error_bytes);
 
 #ifdef __cplusplus
 }

@@ -18,6 +18,9 @@ OK, EINVAL, EUNSUPPORTED, EHIP, ENOMEM = 0, -1, -2, -3, -4
 CHIP_GAUDI, CHIP_GAUDI2, CHIP_GAUDI3 = 0, 1, 2
 # EMmeDataType
 FP8_143, FP8_152, FP16, BF16, FP32, FP32_IEEE, TF32, UFP16 = 9, 10, 11, 12, 13, 14, 15, 17
+# element types of the 8-bit linear layer only (this library's own numbers), and its gates
+INT8, INT32 = 32, 33
+GATE_SILU, GATE_GELU_TANH = 0, 1
 # RoundingMode
 RM_NEAREST_EVEN, RM_TO_ZERO, RM_UP, RM_DOWN, RM_STOCHASTIC, RM_HALF_AWAY, RM_STOCHASTIC_AND_NEAREST = 0, 1, 2, 3, 4, 6, 7
 # EMmeOpType
@@ -27,11 +30,11 @@ FULL_INF_NAN, NO_INF_NAN, MINIMAL_INF_NAN = 0, 1, 2
 REDUCTION_ADD, REDUCTION_SUB, REDUCTION_MIN, REDUCTION_MAX, REDUCTION_MAX_0, REDUCTION_NONE = range(6)  # EMmeReductionOp
 FP8_SPECIALS_CHECK, FP8_SPECIALS_ASSUME_NONE = 0, 1
 
-DTYPE_SIZE = {FP8_143: 1, FP8_152: 1, FP16: 2, UFP16: 2, BF16: 2, FP32: 4, FP32_IEEE: 4, TF32: 4}
+DTYPE_SIZE = {FP8_143: 1, FP8_152: 1, FP16: 2, UFP16: 2, BF16: 2, FP32: 4, FP32_IEEE: 4, TF32: 4, INT8: 1, INT32: 4}
 DTYPE_NUMPY = {FP8_143: np.uint8, FP8_152: np.uint8, BF16: np.uint16, FP16: np.uint16, UFP16: np.uint16, FP32: np.float32,
-               FP32_IEEE: np.float32, TF32: np.uint32}
+               FP32_IEEE: np.float32, TF32: np.uint32, INT8: np.int8, INT32: np.int32}
 DTYPE_NAME = {FP8_143: "fp8_143", FP8_152: "fp8_152", BF16: "bf16", FP16: "fp16", UFP16: "ufp16", FP32: "fp32",
-              FP32_IEEE: "fp32_ieee", TF32: "tf32"}
+              FP32_IEEE: "fp32_ieee", TF32: "tf32", INT8: "int8", INT32: "int32"}
 
 
 class Tensor(C.Structure):
@@ -159,6 +162,10 @@ def load_library():
                                              C.c_size_t] + [C.c_int] * 5
     L.mme_hip_cast_to_fp32_dev.argtypes = [vp, vp, vp, C.c_int, C.c_uint, C.c_int, C.c_size_t, C.c_int, vp, C.c_size_t]
     L.mme_hip_absmax_dev.argtypes = [vp, vp, vp, C.c_size_t]
+    L.mme_hip_quantize_rows_dev.argtypes = [vp, _TP, vp, _TP, _TP, C.c_int]
+    L.mme_hip_rms_norm_quantize_dev.argtypes = [vp, _TP, vp, _TP, _TP, _TP, _TP, C.c_float]
+    L.mme_hip_scaled_gemm_dev.argtypes = [vp, _TP, _TP, vp, _TP, vp, vp]
+    L.mme_hip_plan_scaled_gemm.argtypes = [_TP, _TP, _TP, C.c_int, C.c_int, C.POINTER(C.c_int), C.c_char_p, C.c_size_t]
     _lib = L
     return L
 
@@ -186,4 +193,12 @@ def plan_convolution(out, x, w, y, params, op, epilogue=None, num_cus=256, fp8_s
     form, err = (C.c_int * 4)(), C.create_string_buffer(512)
     rc = lib.mme_hip_plan_convolution(C.byref(out), C.byref(x), C.byref(w), C.byref(y), C.byref(params), op,
                                       C.byref(epilogue) if epilogue is not None else None, num_cus, fp8_specials_policy, form, err, 512)
+    return _planned(rc, form, err)
+
+
+def plan_scaled_gemm(out, x, w, num_cus=256, fp8_specials_policy=FP8_SPECIALS_CHECK):
+    """The same for ``mme_hip_scaled_gemm_dev`` (``mme_hip_plan_scaled_gemm``)."""
+    lib = load_library()
+    form, err = (C.c_int * 4)(), C.create_string_buffer(512)
+    rc = lib.mme_hip_plan_scaled_gemm(C.byref(out), C.byref(x), C.byref(w), num_cus, fp8_specials_policy, form, err, 512)
     return _planned(rc, form, err)

@@ -72,7 +72,32 @@ class MmeSimTensor:
             self._keep = data
             self._ptr = data.data_ptr()
             self.is_device = data.is_cuda
+        self.is_window = False
         self.desc = abi.make_tensor(self._ptr, self.sizes, dtype, fpBias, infNanMode, self.strides, dim)
+
+    def window(self, offset, sizes, strides=None):
+        """A tensor over part of this one's buffer: ``sizes`` elements from element ``offset`` on, with this tensor's strides
+        unless others are given (the gate half and the up half of a projection's output, the heads of a fused one).  For the
+        entry points of the 8-bit linear layer, which touch a tensor's own elements only."""
+        t = object.__new__(MmeSimTensor)
+        t.sizes = list(sizes) + [1] * (abi.MAX_TENSOR_DIMS - len(sizes))
+        t.dim, t.dtype, t.fpBias, t.infNanMode, t.is_device = len(sizes), self.dtype, self.fpBias, self.infNanMode, self.is_device
+        t.strides = list(strides) if strides is not None else list(self.strides)
+        while len(t.strides) < abi.MAX_TENSOR_DIMS:
+            t.strides.append(t.strides[-1] * t.sizes[len(t.strides) - 1])
+        held = self._keep.size if isinstance(self._keep, np.ndarray) else self._keep.numel()
+        first = (self._ptr - self._base()) // abi.DTYPE_SIZE[self.dtype] + offset
+        last = first + sum(st * (sz - 1) for st, sz in zip(t.strides, t.sizes))
+        if offset < 0 or first < 0 or (min(t.sizes) > 0 and last >= held):
+            raise ValueError("the window leaves the tensor's buffer")
+        t._keep, t._ptr, t.is_window = self._keep, self._ptr + offset * abi.DTYPE_SIZE[self.dtype], True
+        t.desc = abi.make_tensor(t._ptr, t.sizes, t.dtype, t.fpBias, t.infNanMode, t.strides, t.dim)
+        for d, st in enumerate(t.strides):  # (a stride of 0 is meant here: the same row for every index)
+            t.desc.strides[d] = st
+        return t
+
+    def _base(self):
+        return self._keep.ctypes.data if isinstance(self._keep, np.ndarray) else self._keep.data_ptr()
 
     # accessors named after the reference's (sim_tensor_base.h:60-90)
     def data(self):
@@ -300,7 +325,50 @@ class HipCalculator:
         self._after_torch(out, src)
         self._check(self._lib.mme_hip_absmax_dev(self._h, out.data_ptr(), src.data_ptr(), n))
 
+    # ---- 8-bit linear layer -------------------------------------------------------------------------------------------
+    def quantizeRows(self, out, rowScales, x, gate=None, gateOp=abi.GATE_SILU):
+        """Rows of ``x`` (or of gate(``gate``) times ``x``) -> 8-bit codes in ``out`` and one fp32 scale per row
+        (mme_hip_quantize_rows_dev).  ``rowScales``: a contiguous float32 torch tensor with one element per row."""
+        self._linear_tensors((out, x, gate), (rowScales,))
+        self._check(self._lib.mme_hip_quantize_rows_dev(self._h, out.desc, self._floats(rowScales, self._rows(out), "rowScales"), x.desc,
+                                                        gate.desc if gate is not None else None, gateOp))
+
+    def rmsNormQuantize(self, out, rowScales, x, gamma=None, residual=None, residualOut=None, eps=1e-6):
+        """Root-mean-square norm of ``x`` (+ ``residual``, the sum kept in ``residualOut``) times ``gamma``, as 8-bit codes and one
+        scale per row (mme_hip_rms_norm_quantize_dev)."""
+        self._linear_tensors((out, x, gamma, residual, residualOut), (rowScales,))
+        self._check(self._lib.mme_hip_rms_norm_quantize_dev(
+            self._h, out.desc, self._floats(rowScales, self._rows(out), "rowScales"), residualOut.desc if residualOut is not None else None, x.desc,
+            residual.desc if residual is not None else None, gamma.desc if gamma is not None else None, eps))
+
+    def scaledGemm(self, out, x, xScales, w, wScales, bias=None):
+        """out = (x w^T) times a scale per row of x and per row of w, plus a bias per row of w, over int8 or fp8 codes
+        (mme_hip_scaled_gemm_dev).  Scales and bias: contiguous float32 torch tensors, or None."""
+        self._linear_tensors((out, x, w), (xScales, wScales, bias))
+        self._check(self._lib.mme_hip_scaled_gemm_dev(self._h, out.desc, x.desc, self._floats(xScales, self._rows(x), "xScales"), w.desc,
+                                                      self._floats(wScales, self._rows(w), "wScales"), self._floats(bias, self._rows(w), "bias")))
+
+    @staticmethod
+    def _rows(t):
+        return t.sizes[1] * t.sizes[2] * t.sizes[3] * t.sizes[4]
+
+    @staticmethod
+    def _floats(t, n, name):
+        if t is None:
+            return None
+        if not t.is_cuda or t.element_size() != 4 or not t.is_floating_point() or not t.is_contiguous() or t.numel() < n:
+            raise MMEStackException("%s: a contiguous float32 device tensor of at least %d elements" % (name, n), abi.EINVAL)
+        return t.data_ptr()
+
+    def _linear_tensors(self, tensors, arrays):
+        for t in tensors:
+            if t is not None and not t.is_device:
+                raise MMEStackException("the 8-bit linear layer needs device tensors", abi.EINVAL)
+        self._after_torch(*[t.data() for t in tensors if t is not None], *arrays)
+
     def _placement(self, *tensors):
+        if any(t.is_window for t in tensors):
+            raise MMEStackException("windows are for the 8-bit linear layer only", abi.EUNSUPPORTED)
         dev = [t.is_device for t in tensors]
         if any(dev) and not all(dev):
             raise MMEStackException("tensors of one call must all be host or all be device resident", abi.EINVAL)

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -16,6 +17,7 @@
 
 #include "../../include/mme_hip.h"
 #include "mme_kernels.hpp"
+#include "scaled_kernels.hpp"
 
 using namespace mme;
 
@@ -96,6 +98,7 @@ struct mme_hip_calc
     void*                 bounce[2] = {nullptr, nullptr};
     hipEvent_t            bounce_ev[2] = {nullptr, nullptr};
     DeviceBuffer          pack_ws[3]; // dense copies of convolution tensors whose strides the kernels cannot follow (weights, dy, output)
+    DeviceBuffer          scaled_ws; // partial sums of the scaled product
     DeviceBuffer          stoch_ws;  // fp32 results of a contraction whose fused epilogue rounds stochastically
     DeviceBuffer          flag;      // one 32-bit cell: epoch number of the latest call whose operands held codes the hardware formats lack
     uint32_t              specials_epoch = 0; // epoch number of the latest call that scanned
@@ -1788,6 +1791,358 @@ int mme_hip_memory_write(mme_hip_handle h, const mme_hip_tensor* memory, const m
     if (int rc = stage_out(h, sm)) return rc;
     HIP_TRY(h, hipStreamSynchronize(h->stream));
     return MME_HIP_OK;
+}
+
+} // extern "C"
+
+// ---------------------------------------------------------------------------------------------------------------------
+// 8-bit linear layer: row quantisers and the scaled product
+// ---------------------------------------------------------------------------------------------------------------------
+namespace
+{
+// The handle's device becomes current for the duration of a call: a launch goes to the current device's context, whatever the
+// stream's device is.
+struct DeviceScope
+{
+    int        old = -1;
+    hipError_t status = hipSuccess;
+    explicit DeviceScope(mme_hip_handle h)
+    {
+        if (h->dry_run) return;
+        status = hipGetDevice(&old);
+        if (status == hipSuccess && old != h->device) status = hipSetDevice(h->device);
+        else
+            old = -1;
+    }
+    ~DeviceScope()
+    {
+        if (old >= 0) (void) hipSetDevice(old);
+    }
+};
+
+// no exception leaves a C entry point (the error text and the retired work spaces allocate)
+template<class F>
+int without_exceptions(mme_hip_handle h, F&& f)
+{
+    if (!h) return MME_HIP_EINVAL;
+    try
+    {
+        note_recording(h);
+        const DeviceScope scope(h);
+        if (scope.status != hipSuccess) return hip_fail(h, scope.status, "hipSetDevice");
+        return f();
+    }
+    catch (...)
+    {
+        return MME_HIP_ENOMEM;
+    }
+}
+
+int linear_elem_size(int dt)
+{
+    switch (dt)
+    {
+        case MME_HIP_INT8:
+        case MME_HIP_FP8_143:
+        case MME_HIP_FP8_152: return 1;
+        case MME_HIP_BF16:
+        case MME_HIP_FP16: return 2;
+        case MME_HIP_FP32:
+        case MME_HIP_INT32: return 4;
+        default: return 0;
+    }
+}
+bool is_code(int dt) { return dt == MME_HIP_INT8 || is_fp8(dt); }
+
+int check_rows_tensor(mme_hip_handle h, const mme_hip_tensor* t, const char* name, bool output)
+{
+    if (!t) return fail(h, MME_HIP_EINVAL, "%s: got null pointer", name);
+    const int es = linear_elem_size(t->dtype);
+    if (es == 0) return fail(h, MME_HIP_EINVAL, "%s: type not supported", name);
+    if (t->strides[0] != 1) return fail(h, MME_HIP_EINVAL, "%s: the first dimension must be contiguous", name);
+    uint64_t n = 1;
+    for (int d = 0; d < 5; d++)
+    {
+        // (stepwise: five 32-bit sizes can overflow 64 bits)
+        n *= t->sizes[d];
+        if (n >= (1ull << 31))
+        {
+            for (int q = d + 1; q < 5; q++)
+                if (t->sizes[q] == 0) n = 0;
+            if (n) return fail(h, MME_HIP_EINVAL, "%s: more than 2^31 elements", name);
+        }
+    }
+    if (n && !t->data) return fail(h, MME_HIP_EINVAL, "%s: got null pointer", name);
+    if (n && (uintptr_t) t->data % es) return fail(h, MME_HIP_EINVAL, "%s: pointer is not aligned to its element type", name);
+    if (t->dtype == MME_HIP_FP16 && (t->fp_bias != 15 || t->inf_nan_mode != MME_HIP_FULL_INF_NAN))
+        return fail(h, MME_HIP_EUNSUPPORTED, "%s: fp16 with exponent bias 15 and full inf/NaN mode only", name);
+    if (output && n)
+    {
+        // rows of an output in the order of their strides: each dimension has to step over everything the smaller ones span
+        int order[4], dims = 0;
+        for (int d = 1; d < 5; d++)
+            if (t->sizes[d] > 1) order[dims++] = d;
+        std::sort(order, order + dims, [&](int a, int b) { return t->strides[a] < t->strides[b]; });
+        uint64_t span = t->sizes[0];
+        for (int i = 0; i < dims; i++)
+        {
+            if (t->strides[order[i]] < span) return fail(h, MME_HIP_EINVAL, "%s: rows overlap", name);
+            span += (uint64_t) t->strides[order[i]] * (t->sizes[order[i]] - 1);
+        }
+    }
+    return MME_HIP_OK;
+}
+
+// bytes from a tensor's first to behind its last element
+uint64_t extent_bytes(const mme_hip_tensor* t)
+{
+    uint64_t last = 0;
+    for (int d = 0; d < 5; d++)
+    {
+        if (t->sizes[d] == 0) return 0;
+        last += (uint64_t) t->strides[d] * (t->sizes[d] - 1);
+    }
+    return (last + 1) * linear_elem_size(t->dtype);
+}
+bool ranges_meet(const void* a, uint64_t na, const void* b, uint64_t nb)
+{
+    const uint64_t pa = (uint64_t) (uintptr_t) a, pb = (uint64_t) (uintptr_t) b;
+    return a && b && na && nb && pa < pb + nb && pb < pa + na;
+}
+bool tensors_meet(const mme_hip_tensor* a, const mme_hip_tensor* b) { return a && b && ranges_meet(a->data, extent_bytes(a), b->data, extent_bytes(b)); }
+bool same_layout(const mme_hip_tensor* a, const mme_hip_tensor* b)
+{
+    if (a->data != b->data || a->dtype != b->dtype) return false;
+    for (int d = 0; d < 5; d++)
+        if (a->sizes[d] != b->sizes[d] || (a->sizes[d] > 1 && a->strides[d] != b->strides[d])) return false;
+    return true;
+}
+int check_float_array(mme_hip_handle h, const void* p, const char* name)
+{
+    if ((uintptr_t) p % 4) return fail(h, MME_HIP_EINVAL, "%s: pointer is not aligned to its element type", name);
+    return MME_HIP_OK;
+}
+int check_fp8_fields(mme_hip_handle h, const mme_hip_tensor* t)
+{
+    if (t->dtype == MME_HIP_FP8_143 && !(t->fp_bias == 3 || t->fp_bias == 7 || t->fp_bias == 11 || t->fp_bias == 15))
+        return fail(h, MME_HIP_EINVAL, "fp8_143 exponent bias must be 3, 7, 11 or 15");
+    if (t->dtype == MME_HIP_FP8_152 && (t->fp_bias < 1 || t->fp_bias > 30)) return fail(h, MME_HIP_EINVAL, "fp8_152 exponent bias must be in 1..30");
+    if (is_fp8(t->dtype) && (t->inf_nan_mode < 0 || t->inf_nan_mode > 2)) return fail(h, MME_HIP_EINVAL, "invalid infNanMode");
+    return MME_HIP_OK;
+}
+
+int quantize_rows(mme_hip_handle h, const mme_hip_tensor* out, float* row_scales, const mme_hip_tensor* sum, const mme_hip_tensor* x,
+                  const mme_hip_tensor* second, const char* second_name, const mme_hip_tensor* gamma, int kind, int gelu, double eps)
+{
+    if (int rc = check_rows_tensor(h, out, "output", true)) return rc;
+    if (int rc = check_rows_tensor(h, x, "x", false)) return rc;
+    if (second)
+        if (int rc = check_rows_tensor(h, second, second_name, false)) return rc;
+    if (sum)
+        if (int rc = check_rows_tensor(h, sum, "residual_out", true)) return rc;
+    if (gamma)
+        if (int rc = check_rows_tensor(h, gamma, "gamma", false)) return rc;
+    if (!is_code(out->dtype)) return fail(h, MME_HIP_EINVAL, "output: int8, fp8_143 or fp8_152");
+    if (int rc = check_fp8_fields(h, out)) return rc;
+    if (out->dtype == MME_HIP_FP8_143 && out->inf_nan_mode == MME_HIP_NO_INF_NAN)
+        return fail(h, MME_HIP_EUNSUPPORTED, "fp8_143 output: full or minimal inf/NaN mode");
+    if (out->dtype == MME_HIP_FP8_152 && out->inf_nan_mode != MME_HIP_FULL_INF_NAN) return fail(h, MME_HIP_EUNSUPPORTED, "fp8_152 output: full inf/NaN mode");
+    if (!(x->dtype == MME_HIP_BF16 || x->dtype == MME_HIP_FP16 || x->dtype == MME_HIP_FP32)) return fail(h, MME_HIP_EINVAL, "x: bf16, fp16 or fp32");
+    for (const mme_hip_tensor* t : {second, sum})
+        if (t && t->dtype != x->dtype) return fail(h, MME_HIP_EINVAL, "%s: type differs from x", t == second ? second_name : "residual_out");
+    for (const mme_hip_tensor* t : {out, second, sum})
+        if (t)
+            for (int d = 0; d < 5; d++)
+                if (t->sizes[d] != x->sizes[d]) return fail(h, MME_HIP_EINVAL, "%s: sizes differ from x", t == out ? "output" : t == second ? second_name : "residual_out");
+    if (gamma)
+    {
+        if (gamma->dtype != x->dtype && gamma->dtype != MME_HIP_FP32) return fail(h, MME_HIP_EINVAL, "gamma: x's type or fp32");
+        if (gamma->sizes[0] != x->sizes[0] || gamma->sizes[1] != 1 || gamma->sizes[2] != 1 || gamma->sizes[3] != 1 || gamma->sizes[4] != 1)
+            return fail(h, MME_HIP_EINVAL, "gamma: one row of x's width");
+    }
+    uint64_t rows = 1;
+    for (int d = 1; d < 5; d++) rows *= x->sizes[d] ? std::min<uint64_t>(x->sizes[d], 1ull << 15) : 0; // (only whether there are any)
+    if (rows == 0) return MME_HIP_OK;
+    if (x->sizes[0] == 0) return fail(h, MME_HIP_EINVAL, "rows of zero elements");
+    rows = n_elements(x) / x->sizes[0];
+    if (!row_scales) return fail(h, MME_HIP_EINVAL, "row_scales: got null pointer");
+    if (int rc = check_float_array(h, row_scales, "row_scales")) return rc;
+    for (const mme_hip_tensor* t : {x, second, gamma})
+        if (t && (tensors_meet(out, t) || ranges_meet(row_scales, rows * 4, t->data, extent_bytes(t)) || (sum && tensors_meet(sum, t) && !(t != gamma && same_layout(sum, t)))))
+            return fail(h, MME_HIP_EINVAL, "an output's memory meets an input's");
+    if (ranges_meet(row_scales, rows * 4, out->data, extent_bytes(out)) || tensors_meet(out, sum) ||
+        (sum && ranges_meet(row_scales, rows * 4, sum->data, extent_bytes(sum))))
+        return fail(h, MME_HIP_EINVAL, "two outputs' memory meets");
+
+    RowQuantArgs a;
+    memset(&a, 0, sizeof a);
+    a.x = x->data;
+    a.second = second ? second->data : nullptr;
+    a.gamma = gamma ? gamma->data : nullptr;
+    a.sum = sum ? sum->data : nullptr;
+    a.codes = (uint8_t*) out->data;
+    a.scales = row_scales;
+    a.rows = (uint32_t) rows;
+    a.width = x->sizes[0];
+    // one stride for all rows where every tensor's dimensions allow it
+    bool flat = true;
+    for (const mme_hip_tensor* t : {x, second, sum, out}) flat = flat && (!t || rows_collapsible(t));
+    for (int d = 0; d < 3; d++) a.n[d] = x->sizes[d + 1];
+    if (flat) a.n[0] = a.rows;
+    auto strides = [&](long long (&st)[4], const mme_hip_tensor* t) {
+        if (!t) return;
+        for (int d = 0; d < 4; d++) st[d] = t->sizes[d + 1] > 1 ? t->strides[d + 1] : 0;
+        if (flat)
+        {
+            // (the pitch of the first dimension that has more than one row: the ones before it have none to step over)
+            int d = 1;
+            while (d < 4 && t->sizes[d] == 1) d++;
+            st[0] = t->strides[d];
+        }
+    };
+    strides(a.x_stride, x);
+    strides(a.second_stride, second);
+    strides(a.sum_stride, sum);
+    strides(a.codes_stride, out);
+    a.kind = kind;
+    auto real = [](int dt) { return dt == MME_HIP_BF16 ? (int) REAL_BF16 : dt == MME_HIP_FP16 ? (int) REAL_FP16 : (int) REAL_FP32; };
+    a.type = real(x->dtype);
+    a.gamma_type = gamma ? real(gamma->dtype) : a.type;
+    a.gelu = gelu;
+    a.code = out->dtype == MME_HIP_INT8 ? CODE_INT8 : out->dtype == MME_HIP_FP8_143 ? CODE_E4M3 : CODE_E5M2;
+    a.qmax = out->dtype == MME_HIP_INT8 ? 127.0f : out->dtype == MME_HIP_FP8_152 ? 57344.0f : out->inf_nan_mode == MME_HIP_FULL_INF_NAN ? 240.0f : 448.0f;
+    a.fold = out->dtype == MME_HIP_INT8 ? 1.0 : pow2f((int) out->fp_bias - (out->dtype == MME_HIP_FP8_143 ? 7 : 15));
+    a.eps = eps;
+    LAUNCH_TRY(h, launch_row_quant(a, h->num_cus, h->stream));
+    return MME_HIP_OK;
+}
+} // namespace
+
+extern "C" {
+
+int mme_hip_quantize_rows_dev(mme_hip_handle h, const mme_hip_tensor* out, float* row_scales, const mme_hip_tensor* x, const mme_hip_tensor* gate, int gate_op)
+{
+    return without_exceptions(h, [&]() -> int {
+        if (gate && gate_op != MME_HIP_GATE_SILU && gate_op != MME_HIP_GATE_GELU_TANH) return fail(h, MME_HIP_EINVAL, "invalid gate %d", gate_op);
+        return quantize_rows(h, out, row_scales, nullptr, x, gate, "gate", nullptr, gate ? ROWS_GATED : ROWS_PLAIN, gate_op == MME_HIP_GATE_GELU_TANH, 0.0);
+    });
+}
+
+int mme_hip_rms_norm_quantize_dev(mme_hip_handle h, const mme_hip_tensor* out, float* row_scales, const mme_hip_tensor* residual_out, const mme_hip_tensor* x,
+                                  const mme_hip_tensor* residual, const mme_hip_tensor* gamma, float eps)
+{
+    return without_exceptions(h, [&]() -> int {
+        if (!(eps >= 0.0f && eps < INFINITY)) return fail(h, MME_HIP_EINVAL, "eps must be finite and not negative");
+        if (residual_out && !residual) return fail(h, MME_HIP_EINVAL, "residual_out without a residual");
+        return quantize_rows(h, out, row_scales, residual_out, x, residual, "residual", gamma, residual ? ROWS_NORM_ADD : ROWS_NORM, 0, (double) eps);
+    });
+}
+
+int mme_hip_scaled_gemm_dev(mme_hip_handle h, const mme_hip_tensor* out, const mme_hip_tensor* x, const float* x_scales, const mme_hip_tensor* w,
+                            const float* w_scales, const float* bias)
+{
+    return without_exceptions(h, [&]() -> int {
+        if (int rc = check_rows_tensor(h, out, "output", true)) return rc;
+        if (int rc = check_rows_tensor(h, x, "x", false)) return rc;
+        if (int rc = check_rows_tensor(h, w, "w", false)) return rc;
+        if (!is_code(x->dtype) || !is_code(w->dtype) || (x->dtype == MME_HIP_INT8) != (w->dtype == MME_HIP_INT8))
+            return fail(h, MME_HIP_EINVAL, "x and w: int8 both, or fp8 both");
+        const bool int8 = x->dtype == MME_HIP_INT8;
+        int        fold = 0;
+        for (const mme_hip_tensor* t : {x, w})
+        {
+            if (int8) continue;
+            if (int rc = check_fp8_fields(h, t)) return rc;
+            if (t->inf_nan_mode != (t->dtype == MME_HIP_FP8_143 ? MME_HIP_MINIMAL_INF_NAN : MME_HIP_FULL_INF_NAN) &&
+                h->fp8_specials_policy != MME_HIP_FP8_SPECIALS_ASSUME_NONE)
+                return fail(h, MME_HIP_EUNSUPPORTED, "%s: this inf/NaN mode needs the promise MME_HIP_FP8_SPECIALS_ASSUME_NONE", t == x ? "x" : "w");
+            fold += (t->dtype == MME_HIP_FP8_143 ? 7 : 15) - (int) t->fp_bias;
+        }
+        const int ot = out->dtype;
+        if (!(ot == MME_HIP_BF16 || ot == MME_HIP_FP16 || ot == MME_HIP_FP32 || (ot == MME_HIP_INT32 && int8)))
+            return fail(h, MME_HIP_EINVAL, "output: bf16, fp16, fp32, or int32 of int8 operands");
+        if (ot == MME_HIP_FP32 && !int8) return fail(h, MME_HIP_EUNSUPPORTED, "output: bf16 or fp16 for fp8 operands, whose sums do not hold what fp32 promises");
+        if (ot == MME_HIP_INT32 && (x_scales || w_scales || bias)) return fail(h, MME_HIP_EINVAL, "int32 output: the sums themselves, without scales and bias");
+        for (int d = 2; d < 5; d++)
+            if (!((x->sizes[d] == out->sizes[d] || x->sizes[d] == 1) && (w->sizes[d] == out->sizes[d] || w->sizes[d] == 1)))
+                return fail(h, MME_HIP_EINVAL, "batch dims doesnt match !");
+        if (x->sizes[0] != w->sizes[0]) return fail(h, MME_HIP_EINVAL, "Common dim doesnt match between input A\\B");
+        if (out->sizes[0] != w->sizes[1]) return fail(h, MME_HIP_EINVAL, "output width doesnt match to inputB width");
+        if (out->sizes[1] != x->sizes[1]) return fail(h, MME_HIP_EINVAL, "output height doesnt match to inputA height");
+        for (int d = 0; d < 5; d++)
+            if (out->sizes[d] == 0) return MME_HIP_OK;
+        if (int8 && x->sizes[0] > 131071u) return fail(h, MME_HIP_EUNSUPPORTED, "int8: a reduction longer than 131071 may overflow its 32-bit sum");
+        if (x->sizes[0] >= (1u << 31)) return fail(h, MME_HIP_EINVAL, "x: more than 2^31 elements");
+        const uint64_t batch = (uint64_t) out->sizes[2] * out->sizes[3] * out->sizes[4];
+        if (batch > 65535u) return fail(h, MME_HIP_EUNSUPPORTED, "more than 65535 batch elements");
+        const uint64_t x_rows = (uint64_t) x->sizes[1] * x->sizes[2] * x->sizes[3] * x->sizes[4], w_rows = (uint64_t) w->sizes[1] * w->sizes[2] * w->sizes[3] * w->sizes[4];
+        const struct
+        {
+            const float* p;
+            uint64_t     bytes;
+            const char*  name;
+        } arrays[3] = {{x_scales, x_rows * 4, "x_scales"}, {w_scales, w_rows * 4, "w_scales"}, {bias, w_rows * 4, "bias"}};
+        for (const auto& s : arrays)
+        {
+            if (int rc = check_float_array(h, s.p, s.name)) return rc;
+            if (ranges_meet(out->data, extent_bytes(out), s.p, s.bytes)) return fail(h, MME_HIP_EINVAL, "an output's memory meets an input's");
+        }
+        // (a planning handle's descriptors carry stand-in addresses)
+        if (!h->dry_run && (tensors_meet(out, x) || tensors_meet(out, w))) return fail(h, MME_HIP_EINVAL, "an output's memory meets an input's");
+
+        ScaledGemmArgs a;
+        memset(&a, 0, sizeof a);
+        a.x = (const uint8_t*) x->data;
+        a.w = (const uint8_t*) w->data;
+        a.out = out->data;
+        a.sx = x_scales;
+        a.sw = w_scales;
+        a.bias = bias;
+        a.M = (int) out->sizes[1];
+        a.N = (int) out->sizes[0];
+        a.K = (int) x->sizes[0];
+        a.x_ld = x->strides[1];
+        a.w_ld = w->strides[1];
+        a.out_ld = out->strides[1];
+        long long sx_step = a.M, sw_step = a.N;
+        for (int d = 0; d < 3; d++)
+        {
+            a.batch[d] = (int) out->sizes[d + 2];
+            a.x_bs[d] = x->sizes[d + 2] == 1 ? 0 : x->strides[d + 2];
+            a.w_bs[d] = w->sizes[d + 2] == 1 ? 0 : w->strides[d + 2];
+            a.out_bs[d] = out->sizes[d + 2] == 1 ? 0 : out->strides[d + 2];
+            a.sx_bs[d] = x->sizes[d + 2] == 1 ? 0 : sx_step;
+            a.sw_bs[d] = w->sizes[d + 2] == 1 ? 0 : sw_step;
+            sx_step *= x->sizes[d + 2];
+            sw_step *= w->sizes[d + 2];
+        }
+        a.int8 = int8;
+        a.fmt = (x->dtype == MME_HIP_FP8_152 ? 1 : 0) | (w->dtype == MME_HIP_FP8_152 ? 2 : 0);
+        a.out_type = ot == MME_HIP_BF16 ? SCALED_OUT_BF16 : ot == MME_HIP_FP16 ? SCALED_OUT_FP16 : ot == MME_HIP_FP32 ? SCALED_OUT_FP32 : SCALED_OUT_INT32;
+        a.alpha = pow2f(fold);
+        plan_scaled_gemm(a, h->num_cus, h->last_form);
+        if (const size_t bytes = scaled_gemm_partial_bytes(a))
+            if (int rc = take_ws(h, h->scaled_ws, bytes, &a.partial)) return rc;
+        LAUNCH_TRY(h, launch_scaled_gemm(a, h->stream));
+        return MME_HIP_OK;
+    });
+}
+
+int mme_hip_plan_scaled_gemm(const mme_hip_tensor* out, const mme_hip_tensor* x, const mme_hip_tensor* w, int num_cus, int fp8_specials_policy, int form[4],
+                             char* error, size_t error_bytes)
+{
+    if (!form) return MME_HIP_EINVAL;
+    try
+    {
+        mme_hip_calc h;
+        make_planning_handle(h, num_cus, fp8_specials_policy);
+        h.last_form[0] = -1;
+        return planned_form(h, mme_hip_scaled_gemm_dev(&h, out, x, nullptr, w, nullptr, nullptr), form, error, error_bytes);
+    }
+    catch (...)
+    {
+        return MME_HIP_ENOMEM;
+    }
 }
 
 } // extern "C"

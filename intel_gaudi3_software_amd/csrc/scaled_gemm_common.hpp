@@ -1,0 +1,134 @@
+// scaled_gemm_common.hpp -- what the kernels of the scaled product share:
+//   out[m][n] = (sum_k x[m][k] w[n][k]) sx[m] sw[n] + bias[n]
+// over int8 codes (sums in int32, exact) or fp8 codes (sums in fp32).  The matrix-core instructions take the rows of w first, so
+// that an accumulator register group runs along n: lane l holds token l % 32 (or l % 16) and four consecutive n at a time.
+#pragma once
+#include <type_traits>
+
+#include "mme_numeric.hpp"
+#include "scaled_kernels.hpp"
+
+namespace mme
+{
+namespace
+{
+typedef int   s_v4i __attribute__((ext_vector_type(4)));
+typedef int   s_v8i __attribute__((ext_vector_type(8)));
+typedef int   s_v16i __attribute__((ext_vector_type(16)));
+typedef float s_v4f __attribute__((ext_vector_type(4)));
+typedef float s_v16f __attribute__((ext_vector_type(16)));
+
+// OPS: -1 int8; 0 .. 3 fp8, bit 0: x is e5m2, bit 1: w is e5m2
+template<int OPS>
+struct Sums
+{
+    typedef s_v16f v16;
+    typedef s_v4f  v4;
+    typedef float  one;
+};
+template<>
+struct Sums<-1>
+{
+    typedef s_v16i v16;
+    typedef s_v4i  v4;
+    typedef int    one;
+};
+
+// 32 rows of w x 32 rows of x over 64 k: lane l holds 32 codes of row l % 32; which k they are does not matter as long as both
+// operands agree.  int8: two instructions of 32 k, the lower and the upper half of the registers.
+template<int OPS>
+__device__ __forceinline__ typename Sums<OPS>::v16 mma32(s_v8i w, s_v8i x, typename Sums<OPS>::v16 c)
+{
+    if constexpr (OPS < 0)
+    {
+        c = __builtin_amdgcn_mfma_i32_32x32x32_i8(s_v4i {w[0], w[1], w[2], w[3]}, s_v4i {x[0], x[1], x[2], x[3]}, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_i32_32x32x32_i8(s_v4i {w[4], w[5], w[6], w[7]}, s_v4i {x[4], x[5], x[6], x[7]}, c, 0, 0, 0);
+    }
+    else
+        return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, (OPS >> 1) & 1, OPS & 1, 0, 0, 0, 0);
+}
+// 16 x 16 over 128 k: lane l holds 32 codes of row l % 16
+template<int OPS>
+__device__ __forceinline__ typename Sums<OPS>::v4 mma16(s_v8i w, s_v8i x, typename Sums<OPS>::v4 c)
+{
+    if constexpr (OPS < 0)
+    {
+        c = __builtin_amdgcn_mfma_i32_16x16x64_i8(s_v4i {w[0], w[1], w[2], w[3]}, s_v4i {x[0], x[1], x[2], x[3]}, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(s_v4i {w[4], w[5], w[6], w[7]}, s_v4i {x[4], x[5], x[6], x[7]}, c, 0, 0, 0);
+    }
+    else
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, (OPS >> 1) & 1, OPS & 1, 0, 0, 0, 0);
+}
+
+struct BatchOffsets
+{
+    long long x, w, out, sx, sw;
+};
+__device__ __forceinline__ BatchOffsets batch_offsets(const ScaledGemmArgs& a, int b)
+{
+    const int b0 = b % a.batch[0], r = b / a.batch[0], b1 = r % a.batch[1], b2 = r / a.batch[1];
+    auto at = [&](const long long (&st)[3]) { return b0 * st[0] + b1 * st[1] + b2 * st[2]; };
+    return BatchOffsets {at(a.x_bs), at(a.w_bs), at(a.out_bs), at(a.sx_bs), at(a.sw_bs)};
+}
+
+// the value that is rounded into the output: one rounding of a whole sum to fp32, two multiplications, one addition, each rounded
+// once (the factors one after the other: their product may leave the fp32 range where the result does not)
+template<class S>
+__device__ __forceinline__ float scaled_value(S sum, float alpha, float sx, float sw, float bias, bool has_bias)
+{
+    float v = (float) sum;
+    if constexpr (std::is_same<S, float>::value) v *= alpha;
+    v *= sx;
+    return has_bias ? __builtin_fmaf(v, sw, bias) : v * sw;
+}
+__device__ __forceinline__ uint16_t to_half(float v, int out_type)
+{
+    uint16_t u;
+    if (out_type == SCALED_OUT_BF16)
+    {
+        const __bf16 h = (__bf16) v;
+        __builtin_memcpy(&u, &h, 2);
+    }
+    else
+    {
+        const _Float16 h = (_Float16) v;
+        __builtin_memcpy(&u, &h, 2);
+    }
+    return u;
+}
+
+// stores four consecutive outputs n .. n + 3 of row m (those below N), from their sums
+template<class S>
+__device__ __forceinline__ void store_scaled4(const ScaledGemmArgs& a, const BatchOffsets& o, int m, int n, const S (&sum)[4])
+{
+    const long long e = o.out + (long long) m * a.out_ld + n;
+    if (a.out_type == SCALED_OUT_INT32)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (n + i < a.N) ((int*) a.out)[e + i] = (int) sum[i];
+        return;
+    }
+    const float sx = a.sx ? a.sx[o.sx + m] : 1.0f;
+    float       v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+    {
+        const int q = min(n + i, a.N - 1);
+        v[i] = scaled_value(sum[i], a.alpha, sx, a.sw ? a.sw[o.sw + q] : 1.0f, a.bias ? a.bias[o.sw + q] : 0.0f, a.bias != nullptr);
+    }
+    if (a.out_type == SCALED_OUT_FP32)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (n + i < a.N) ((float*) a.out)[e + i] = v[i];
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (n + i < a.N) ((uint16_t*) a.out)[e + i] = to_half(v[i], a.out_type);
+    }
+}
+} // namespace
+} // namespace mme
