@@ -358,7 +358,9 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(const RowQ
     // an inf or NaN among s shows in the squares' sum as well as in u unless gamma is zero there
     const bool  bad = top >= INF_BITS || (NORM && !(sum < __uint_as_float(INF_BITS)));
     const float most = __uint_as_float(top);
+    // qmax / max|u| in two parts, f the quotient rounded to fp32, f_lo what that leaves out
     const float f = bad || top == 0u ? 0.0f : a.qmax / most;
+    const float f_lo = bad || top == 0u ? 0.0f : __builtin_fmaf(-f, most, a.qmax) / most;
 
     const long long c0 = at(a.codes_stride);
     auto            put = [&](int n, int e) __attribute__((always_inline))
@@ -370,17 +372,19 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(const RowQ
         if (!bad)
         {
             float q[VEC];
+            if (a.code != CODE_INT8)
 #pragma unroll
-            for (int i = 0; i < VEC; i++) q[i] = __builtin_amdgcn_fmed3f(u[n][i] * f, -a.qmax, a.qmax);
+                for (int i = 0; i < VEC; i++) q[i] = __builtin_amdgcn_fmed3f(__builtin_fmaf(u[n][i], f, u[n][i] * f_lo), -a.qmax, a.qmax);
             if (a.code == CODE_INT8)
             {
-                // adding 1.5 x 2^23 rounds to a whole number, whose two's complement stands in the low byte
+                // added to 1.5 x 2^23 the product is rounded once, to a whole number (127 for the largest: f is off by less than
+                // 2^-24), whose two's complement stands in the low byte
 #pragma unroll
                 for (int h = 0; h < 2; h++)
                 {
                     uint32_t b[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) b[i] = __float_as_uint(q[4 * h + i] + 12582912.0f);
+                    for (int i = 0; i < 4; i++) b[i] = __float_as_uint(__builtin_fmaf(u[n][4 * h + i], f, 12582912.0f));
                     const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000C0Cu);
                     c[h] = lo | hi;
                 }

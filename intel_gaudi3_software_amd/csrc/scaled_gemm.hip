@@ -4,32 +4,16 @@
 // General form: 64 x 64 outputs per workgroup of four wavefronts (2 x 2, 32 x 32 each), 64 k per step.  Operands go through
 // registers into LDS (rows of 64 codes on a pitch of 80 bytes), loaded 16 bytes at a time at any alignment; codes beyond K are
 // replaced by zeros in both operands, so that nothing behind a row's end reaches a sum.
+#include <mutex>
+#include <utility>
+#include <vector>
+
 #include "scaled_gemm_common.hpp"
 
 namespace mme
 {
 namespace
 {
-struct __attribute__((packed, aligned(1))) u128_any
-{
-    uint32_t v[4];
-};
-
-// 16 codes of a row from k on, zeros behind the row's end
-__device__ __forceinline__ s_v4i load16(const uint8_t* row, int k, int K)
-{
-    if (k + 16 <= K)
-    {
-        const u128_any u = *(const u128_any*) (row + k);
-        return s_v4i {(int) u.v[0], (int) u.v[1], (int) u.v[2], (int) u.v[3]};
-    }
-    uint32_t v[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < 16; i++)
-        if (k + i < K) v[i / 4] |= (uint32_t) row[k + i] << (8 * (i & 3));
-    return s_v4i {(int) v[0], (int) v[1], (int) v[2], (int) v[3]};
-}
-
 constexpr int GT = 64, GK = 64, GP = 80;
 
 template<int OPS>
@@ -61,8 +45,7 @@ __global__ __launch_bounds__(256) void scaled_gemm_general_kernel(const ScaledGe
         auto frag = [&](const char* base, int row) __attribute__((always_inline))
         {
             const char* p = base + (row + (lane & 31)) * GP + (lane >> 5) * 32;
-            const s_v4i lo = *(const s_v4i*) p, hi = *(const s_v4i*) (p + 16);
-            return s_v8i {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            return join(*(const s_v4i*) p, *(const s_v4i*) (p + 16));
         };
         acc = mma32<OPS>(frag(lds[1], wn * 32), frag(lds[0], wm * 32), acc);
         __syncthreads();
@@ -79,12 +62,34 @@ __global__ __launch_bounds__(256) void scaled_gemm_general_kernel(const ScaledGe
 }
 } // namespace
 
+hipError_t allow_lds(const void* kernel, int bytes)
+{
+    static std::mutex                               mutex;
+    static std::vector<std::pair<const void*, int>> done;
+    int                                             device = 0;
+    if (hipError_t e = hipGetDevice(&device)) return e;
+    const std::lock_guard<std::mutex> lock(mutex);
+    for (const auto& d : done)
+        if (d.first == kernel && d.second == device) return hipSuccess;
+    if (hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    done.emplace_back(kernel, device);
+    return hipSuccess;
+}
+
 void plan_scaled_gemm(ScaledGemmArgs& a, int num_cus, int (&figures)[4])
 {
-    (void) num_cus;
     a.form = SCALED_FORM_GENERAL;
     a.split_k = 1;
     figures[0] = 0, figures[1] = GT, figures[2] = 1, figures[3] = 4;
+    bool aligned = (uintptr_t) a.x % 16 == 0 && (uintptr_t) a.w % 16 == 0 && (a.M == 1 || a.x_ld % 16 == 0) && (a.N == 1 || a.w_ld % 16 == 0);
+    for (int d = 0; d < 3; d++) aligned = aligned && a.x_bs[d] % 16 == 0 && a.w_bs[d] % 16 == 0;
+    a.aligned = aligned;
+    if (a.M <= 32)
+    {
+        a.form = SCALED_FORM_FEW;
+        scaled_gemm_few_shape(a, num_cus);
+        figures[0] = 3, figures[1] = a.tile_m, figures[3] = a.waves;
+    }
 }
 
 size_t scaled_gemm_partial_bytes(const ScaledGemmArgs& a)
@@ -94,6 +99,7 @@ size_t scaled_gemm_partial_bytes(const ScaledGemmArgs& a)
 
 hipError_t launch_scaled_gemm(const ScaledGemmArgs& a, hipStream_t s)
 {
+    if (a.form == SCALED_FORM_FEW) return launch_scaled_gemm_few(a, s);
     const dim3 grid((unsigned) (((a.M + GT - 1) / GT) * ((a.N + GT - 1) / GT)), (unsigned) (a.batch[0] * a.batch[1] * a.batch[2]));
     auto       go = [&](auto ops) { hipLaunchKernelGGL((scaled_gemm_general_kernel<decltype(ops)::value>), grid, dim3(256), 0, s, a); };
     if (a.int8) go(std::integral_constant<int, -1>());

@@ -60,6 +60,38 @@ __device__ __forceinline__ typename Sums<OPS>::v4 mma16(s_v8i w, s_v8i x, typena
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, (OPS >> 1) & 1, OPS & 1, 0, 0, 0, 0);
 }
 
+struct __attribute__((packed, aligned(1))) u128_any
+{
+    uint32_t v[4];
+};
+
+// 16 codes of a row from k on, at any alignment, zeros behind the row's end
+__device__ __forceinline__ s_v4i load16(const uint8_t* row, int k, int K)
+{
+    if (k + 16 <= K)
+    {
+        const u128_any u = *(const u128_any*) (row + k);
+        return s_v4i {(int) u.v[0], (int) u.v[1], (int) u.v[2], (int) u.v[3]};
+    }
+    if (k >= K) return s_v4i {0, 0, 0, 0};
+    if (K >= 16)
+    {
+        // the row's last sixteen codes, moved down by those that come before k
+        const u128_any     u = *(const u128_any*) (row + K - 16);
+        const int          bits = 8 * (k + 16 - K); // 8 .. 120
+        unsigned long long lo = ((unsigned long long) u.v[1] << 32) | u.v[0], hi = ((unsigned long long) u.v[3] << 32) | u.v[2];
+        lo = bits >= 64 ? hi >> (bits & 63) : (lo >> bits) | (hi << (64 - bits));
+        hi = bits >= 64 ? 0ull : hi >> bits;
+        return s_v4i {(int) (uint32_t) lo, (int) (uint32_t) (lo >> 32), (int) (uint32_t) hi, (int) (uint32_t) (hi >> 32)};
+    }
+    uint32_t v[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+        if (k + i < K) v[i / 4] |= (uint32_t) row[k + i] << (8 * (i & 3));
+    return s_v4i {(int) v[0], (int) v[1], (int) v[2], (int) v[3]};
+}
+__device__ __forceinline__ s_v8i join(s_v4i lo, s_v4i hi) { return s_v8i {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}; }
+
 struct BatchOffsets
 {
     long long x, w, out, sx, sw;

@@ -76,18 +76,26 @@ struct ScaledGemmArgs
     int            fmt;     // fp8: bit 0 = x is e5m2, bit 1 = w is e5m2
     int            out_type;
     float          alpha;   // fp8: power of two of the exponent biases
+    int            aligned; // every row of x and w starts at a multiple of 16 bytes
     int            form;    // SCALED_FORM_*, filled in by plan_scaled_gemm
+    int            tile_m, tile_n; // shape of a workgroup's outputs, in the form's own units
+    int            waves;   // wavefronts per workgroup
     int            split_k; // slices of the reduction, 1: none
     void*          partial; // split_k > 1: split_k x batch x M x N sums (int32 / fp32)
 };
 
 enum : int
 {
-    SCALED_FORM_GENERAL = 0
+    SCALED_FORM_GENERAL = 0,
+    SCALED_FORM_FEW = 1 // few rows of x (scaled_gemm_few.hip)
 };
 
 // picks the kernel form and the slices of the reduction for these operands; figures: what mme_hip_last_contraction_form reports
 void       plan_scaled_gemm(ScaledGemmArgs& a, int num_cus, int (&figures)[4]);
 size_t     scaled_gemm_partial_bytes(const ScaledGemmArgs& a);
+// lets a kernel have `bytes` of dynamic LDS on the current device (asked for once per kernel and device)
+hipError_t allow_lds(const void* kernel, int bytes);
+void       scaled_gemm_few_shape(ScaledGemmArgs& a, int num_cus);
+hipError_t launch_scaled_gemm_few(const ScaledGemmArgs& a, hipStream_t s);
 hipError_t launch_scaled_gemm(const ScaledGemmArgs& a, hipStream_t s);
 } // namespace mme
