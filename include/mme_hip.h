@@ -526,8 +526,8 @@ int mme_hip_absmax_dev(mme_hip_handle h, float* out_absmax, const float* in, siz
 /*
  * A linear layer in 8 bits with a scale per token and per output channel (no counterpart in the reference, whose scales are
  * exponent biases and powers of two): the quantisers turn rows of values into rows of codes and one fp32 scale each, the product
- * multiplies codes by codes and applies the scales.  All three take device pointers, enqueue one kernel (the product two where
- * it splits a reduction) on the handle's stream, whichever device is current, and can be recorded into a graph.
+ * multiplies codes by codes and applies the scales.  All three take device pointers, enqueue one kernel on the handle's stream,
+ * whichever device is current, use no work space and allocate nothing, and can be recorded into a graph.
  *
  * A row is dimension 0 of a tensor (sizes[0] elements, contiguous); dimensions 1 .. 4 enumerate rows, with any strides.
  * Input rows may share memory (stride 0: the same row for every index); output rows may not, and an output's memory
@@ -585,10 +585,8 @@ int mme_hip_rms_norm_quantize_dev(mme_hip_handle        h,
  *     code has all exponent bits set, which holds for what the quantisers write: EUNSUPPORTED without it.
  * The sum is rounded to fp32, multiplied by the scale of x, then by that of w (together with the addition of the bias in one
  * rounding), then rounded to nearest even into out's type; out of range becomes inf.  fp16 outputs have exponent bias 15.
- * The result does not depend on which rows are computed together nor on timing: it is the same for every call with the same operands and
- * sizes.  K = 0 gives the bias.  Up to 65535 batch elements.
- * With a split reduction the partial sums go to a work space of the handle (see mme_hip_set_stream; for recording, see
- * mme_hip_batch_gemm_dev_noalloc: call once with these sizes before the recording starts).
+ * The result is the same, bit for bit, for every call with the same operands, sizes and strides.  K = 0 gives the bias.  Up to 65535
+ * batch elements.
  */
 int mme_hip_scaled_gemm_dev(mme_hip_handle        h,
                             const mme_hip_tensor* out,
@@ -599,9 +597,8 @@ int mme_hip_scaled_gemm_dev(mme_hip_handle        h,
                             const float*          bias);    /* may be NULL */
 
 /*
- * What mme_hip_scaled_gemm_dev would launch for these descriptors, like mme_hip_plan_batch_gemm: form[0] 0 the general kernel, 1 a
- * tile kernel, 3 the kernel for few rows of x; form[1] rows of x per workgroup; form[2] slices of the reduction; form[3] wavefronts
- * per workgroup.  mme_hip_last_contraction_form reports the same after a call.
+ * What mme_hip_scaled_gemm_dev would launch for these descriptors, like mme_hip_plan_batch_gemm: form[0] 1 a tile kernel, 3
+ * the kernel for few rows of x; form[1] rows of x per workgroup; form[2] 1 (the reduction is never split); form[3] wavefronts per workgroup.  mme_hip_last_contraction_form reports the same after a call.
  */
 int mme_hip_plan_scaled_gemm(const mme_hip_tensor* out, const mme_hip_tensor* x, const mme_hip_tensor* w, int num_cus, int fp8_specials_policy,
                              int form[4], char* error, size_t error_bytes);

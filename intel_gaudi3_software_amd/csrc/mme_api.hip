@@ -98,7 +98,6 @@ struct mme_hip_calc
     void*                 bounce[2] = {nullptr, nullptr};
     hipEvent_t            bounce_ev[2] = {nullptr, nullptr};
     DeviceBuffer          pack_ws[3]; // dense copies of convolution tensors whose strides the kernels cannot follow (weights, dy, output)
-    DeviceBuffer          scaled_ws; // partial sums of the scaled product
     DeviceBuffer          stoch_ws;  // fp32 results of a contraction whose fused epilogue rounds stochastically
     DeviceBuffer          flag;      // one 32-bit cell: epoch number of the latest call whose operands held codes the hardware formats lack
     uint32_t              specials_epoch = 0; // epoch number of the latest call that scanned
@@ -2121,8 +2120,6 @@ int mme_hip_scaled_gemm_dev(mme_hip_handle h, const mme_hip_tensor* out, const m
         a.out_type = ot == MME_HIP_BF16 ? SCALED_OUT_BF16 : ot == MME_HIP_FP16 ? SCALED_OUT_FP16 : ot == MME_HIP_FP32 ? SCALED_OUT_FP32 : SCALED_OUT_INT32;
         a.alpha = pow2f(fold);
         plan_scaled_gemm(a, h->num_cus, h->last_form);
-        if (const size_t bytes = scaled_gemm_partial_bytes(a))
-            if (int rc = take_ws(h, h->scaled_ws, bytes, &a.partial)) return rc;
         LAUNCH_TRY(h, launch_scaled_gemm(a, h->stream));
         return MME_HIP_OK;
     });

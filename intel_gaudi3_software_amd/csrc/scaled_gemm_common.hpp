@@ -92,6 +92,17 @@ __device__ __forceinline__ s_v4i load16(const uint8_t* row, int k, int K)
 }
 __device__ __forceinline__ s_v8i join(s_v4i lo, s_v4i hi) { return s_v8i {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}; }
 
+// 16 bytes per lane from global memory to LDS at lds_off + lane * 16 (lds_off is wave-uniform), outside the compiler's memory model:
+// the wavefront waits for its requests by count
+__device__ __forceinline__ void dma16(const void* g, uint32_t lds_off)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_off) : "memory");
+}
+// where a row of 128 bytes keeps its 16-byte chunk c: at c ^ swizzle(row).  A line of all LDS banks holds two rows, so sixteen rows with
+// the same c meet every bank once.
+__device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
+constexpr int vm_wait(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); } // at most n of the wavefront's requests outstanding
+
 struct BatchOffsets
 {
     long long x, w, out, sx, sw;
@@ -129,38 +140,74 @@ __device__ __forceinline__ uint16_t to_half(float v, int out_type)
     return u;
 }
 
-// stores four consecutive outputs n .. n + 3 of row m (those below N), from their sums
+struct __attribute__((packed, aligned(1))) u64_any
+{
+    uint32_t v[2];
+};
+struct __attribute__((packed, aligned(4))) f128_any
+{
+    float v[4];
+};
+
+// stores four consecutive outputs n .. n + 3 of row m (those below N), from their sums; sx: the row's scale
 template<class S>
-__device__ __forceinline__ void store_scaled4(const ScaledGemmArgs& a, const BatchOffsets& o, int m, int n, const S (&sum)[4])
+__device__ __forceinline__ void store_scaled4(const ScaledGemmArgs& a, const BatchOffsets& o, int m, int n, float sx, const S (&sum)[4])
 {
     const long long e = o.out + (long long) m * a.out_ld + n;
+    const bool      whole = n + 4 <= a.N;
+    uint32_t        word[4];
     if (a.out_type == SCALED_OUT_INT32)
     {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (n + i < a.N) ((int*) a.out)[e + i] = (int) sum[i];
-        return;
-    }
-    const float sx = a.sx ? a.sx[o.sx + m] : 1.0f;
-    float       v[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-    {
-        const int q = min(n + i, a.N - 1);
-        v[i] = scaled_value(sum[i], a.alpha, sx, a.sw ? a.sw[o.sw + q] : 1.0f, a.bias ? a.bias[o.sw + q] : 0.0f, a.bias != nullptr);
-    }
-    if (a.out_type == SCALED_OUT_FP32)
-    {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (n + i < a.N) ((float*) a.out)[e + i] = v[i];
+        for (int i = 0; i < 4; i++) word[i] = (uint32_t) (int) sum[i];
     }
     else
     {
+        f128_any sw = {{1.0f, 1.0f, 1.0f, 1.0f}}, bias = {{0.0f, 0.0f, 0.0f, 0.0f}};
+        if (whole)
+        {
+            if (a.sw) sw = *(const f128_any*) (a.sw + o.sw + n);
+            if (a.bias) bias = *(const f128_any*) (a.bias + o.sw + n);
+        }
+        else
+        {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (n + i < a.N) ((uint16_t*) a.out)[e + i] = to_half(v[i], a.out_type);
+            for (int i = 0; i < 4; i++)
+            {
+                const int q = min(n + i, a.N - 1);
+                if (a.sw) sw.v[i] = a.sw[o.sw + q];
+                if (a.bias) bias.v[i] = a.bias[o.sw + q];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) word[i] = __float_as_uint(scaled_value(sum[i], a.alpha, sx, sw.v[i], bias.v[i], a.bias != nullptr));
+    }
+    if (a.out_type == SCALED_OUT_FP32 || a.out_type == SCALED_OUT_INT32)
+    {
+        uint32_t* p = (uint32_t*) a.out + e;
+        if (whole) *(u128_any*) p = u128_any {{word[0], word[1], word[2], word[3]}};
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (n + i < a.N) p[i] = word[i];
+        }
+    }
+    else
+    {
+        uint16_t* p = (uint16_t*) a.out + e;
+        uint32_t  half[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) half[i] = to_half(__uint_as_float(word[i]), a.out_type);
+        if (whole) *(u64_any*) p = u64_any {{half[0] | (half[1] << 16), half[2] | (half[3] << 16)}};
+        else
+        {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (n + i < a.N) p[i] = (uint16_t) half[i];
+        }
     }
 }
+__device__ __forceinline__ float scale_of_row(const ScaledGemmArgs& a, const BatchOffsets& o, int m) { return a.sx ? a.sx[o.sx + min(m, a.M - 1)] : 1.0f; }
 } // namespace
 } // namespace mme

@@ -1,12 +1,12 @@
-// scaled_gemm_few.hip -- the scaled product for few rows of x (tokens being generated): up to 32.
+// scaled_gemm_few.hip -- the scaled product for few rows of x (tokens being generated), or few outputs in all.
 //
-// Bound by reading w once.  A workgroup owns 16 NT rows of w and all rows of x; its wavefronts share out the reduction, 128 k at a
+// Bound by reading w once.  A workgroup owns 16 NT rows of w and 8, 16 or 32 rows of x; its wavefronts share out the reduction, 128 k at a
 // time in turn, and share nothing until the end, when their partial sums meet in LDS and are added in the order of the wavefronts.
 //
 // The 16 x 16 matrix instructions want neighbouring lanes on neighbouring rows.  Loaded that way from memory every lane is a line
 // of its own and a compute unit takes in 17 bytes a clock; so a wavefront brings a stage (128 k of every row) into a ring of its
 // own in LDS, eight neighbouring lanes on the eight 16-byte chunks of a line, and reads it back in the instructions' layout (chunk c of
-// row r lies at position c ^ (r & 7): no bank is met twice).  Sixteen tokens, 4096 x 14336: 11.9 us, 4.9 TB/s of w and x (loaded straight into
+// row r lies at position c ^ (r / 2 & 7): the sixteen rows of a read meet every bank once).  Sixteen tokens, 4096 x 14336: 11.9 us, 4.9 TB/s of w and x (loaded straight into
 // the instructions' layout: 15.2); 14336 x 4096: 12.5 us, 4.7 TB/s; one token, 4096 x 4096: 5.7 us, most of it the launch.  Where all rows are 16-byte aligned the copies are direct, memory to
 // LDS, and D stages are in flight; elsewhere they pass through registers.  The last K % 128 codes are loaded by hand.
 #include "scaled_gemm_common.hpp"
@@ -15,14 +15,6 @@ namespace mme
 {
 namespace
 {
-// 16 bytes per lane from global memory to LDS at lds_off + lane * 16 (lds_off is wave-uniform), outside the compiler's memory model:
-// the wavefront waits for its requests by count
-__device__ __forceinline__ void dma16(const void* g, uint32_t lds_off)
-{
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_off) : "memory");
-}
-constexpr int vm_wait(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); } // at most n of the wavefront's requests outstanding
-
 // NT: 16-row tiles of w; XR: rows of x (8, 16 or 32); D: stages of a wavefront's ring
 template<int OPS, int NT, int XR, int WAVES, int D, bool ALIGNED>
 __global__ __launch_bounds__(WAVES * 64) void scaled_gemm_few_kernel(const ScaledGemmArgs a)
@@ -34,9 +26,13 @@ __global__ __launch_bounds__(WAVES * 64) void scaled_gemm_few_kernel(const Scale
     constexpr int STAGE = Q * 1024;
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     const int          lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int          n0 = (int) blockIdx.x * (16 * NT);
+    // consecutive tiles go to one XCD (workgroups are dealt out to the eight in turn), those over one panel of w next to each other
+    const int tiles_m = (a.M + XR - 1) / XR, total = (int) gridDim.x, xcd = (int) blockIdx.x & 7;
+    const int tile = xcd * (total >> 3) + min(xcd, total & 7) + ((int) blockIdx.x >> 3);
+    const int m0 = (tile % tiles_m) * XR, n0 = (tile / tiles_m) * (16 * NT);
     const BatchOffsets o = batch_offsets(a, blockIdx.y);
-    const int          row8 = lane >> 3, chunk = (lane & 7) ^ row8; // request side: row of eight, the 16-byte chunk of its line
+    const int          row8 = lane >> 3; // request side: row of eight
+    auto chunk = [&](int q) __attribute__((always_inline)) { return (lane & 7) ^ swizzle(q * 8 + row8); }; // and the 16-byte chunk of its line
     char*              ring = lds + wave * (D * STAGE);
     const uint32_t     ring_off = (uint32_t) (uintptr_t) lds + wave * (D * STAGE);
     const uint8_t*     w = a.w + o.w;
@@ -44,9 +40,9 @@ __global__ __launch_bounds__(WAVES * 64) void scaled_gemm_few_kernel(const Scale
     // (rows beyond the last read the last: their outputs are not stored)
     const uint8_t* src[Q];
 #pragma unroll
-    for (int q = 0; q < QW; q++) src[q] = w + (long long) min(n0 + q * 8 + row8, a.N - 1) * a.w_ld + chunk * 16 + wave * 128;
+    for (int q = 0; q < QW; q++) src[q] = w + (long long) min(n0 + q * 8 + row8, a.N - 1) * a.w_ld + chunk(q) * 16 + wave * 128;
 #pragma unroll
-    for (int q = 0; q < QX; q++) src[QW + q] = x + (long long) min(q * 8 + row8, a.M - 1) * a.x_ld + chunk * 16 + wave * 128;
+    for (int q = 0; q < QX; q++) src[QW + q] = x + (long long) min(m0 + q * 8 + row8, a.M - 1) * a.x_ld + chunk(q) * 16 + wave * 128;
 
     v4 acc[MT][NT];
 #pragma unroll
@@ -65,7 +61,7 @@ __global__ __launch_bounds__(WAVES * 64) void scaled_gemm_few_kernel(const Scale
         auto frag = [&](int row) __attribute__((always_inline))
         {
             const char* p = st + row * 128;
-            return join(*(const s_v4i*) (p + ((g ^ (row & 7)) << 4)), *(const s_v4i*) (p + (((g + 4) ^ (row & 7)) << 4)));
+            return join(*(const s_v4i*) (p + ((g ^ swizzle(row)) << 4)), *(const s_v4i*) (p + (((g + 4) ^ swizzle(row)) << 4)));
         };
         s_v8i fw[NT], fx[MT];
 #pragma unroll
@@ -145,7 +141,7 @@ __global__ __launch_bounds__(WAVES * 64) void scaled_gemm_few_kernel(const Scale
 #pragma unroll
         for (int i = 0; i < MT; i++)
         {
-            const uint8_t* p = x + (long long) min(i * 16 + r, a.M - 1) * a.x_ld;
+            const uint8_t* p = x + (long long) min(m0 + i * 16 + r, a.M - 1) * a.x_ld;
             fx[i] = join(load16(p, k, a.K), load16(p, k + 64, a.K));
         }
 #pragma unroll
@@ -164,14 +160,18 @@ __global__ __launch_bounds__(WAVES * 64) void scaled_gemm_few_kernel(const Scale
 #pragma unroll
         for (int j = 0; j < NT; j++) *(v4*) (part + ((wave * MT * NT + i * NT + j) * 64 + lane) * 4) = acc[i][j];
     __syncthreads();
+    // consecutive lanes on consecutive groups of four columns of a row
     for (int t = threadIdx.x; t < MT * NT * 64; t += WAVES * 64)
     {
-        const int tile = t >> 6, l = t & 63, m = (tile / NT) * 16 + (l & 15), n = n0 + (tile % NT) * 16 + 4 * (l >> 4);
-        v4        sum = *(const v4*) (part + (tile * 64 + l) * 4);
+        const int row = t / (4 * NT), group = t % (4 * NT), l = (group & 3) * 16 + (row & 15), block = (row >> 4) * NT + (group >> 2);
+        const int m = m0 + row, n = n0 + group * 4;
+        if (m >= a.M || n >= a.N) continue;
+        const float sx = scale_of_row(a, o, m);
+        v4          sum = *(const v4*) (part + (block * 64 + l) * 4);
 #pragma unroll
-        for (int q = 1; q < WAVES; q++) sum += *(const v4*) (part + ((q * MT * NT + tile) * 64 + l) * 4);
+        for (int q = 1; q < WAVES; q++) sum += *(const v4*) (part + ((q * MT * NT + block) * 64 + l) * 4);
         const one s[4] = {sum[0], sum[1], sum[2], sum[3]};
-        if (m < a.M && n < a.N) store_scaled4(a, o, m, n, s);
+        store_scaled4(a, o, m, n, sx, s);
     }
 }
 
@@ -182,7 +182,7 @@ hipError_t start(const ScaledGemmArgs& a, hipStream_t s)
     constexpr int ring = WAVES * D * (16 * NT + XR) * 128, sums = WAVES * MT * NT * 1024, lds = ring > sums ? ring : sums;
     static_assert(lds <= 160 * 1024, "LDS of a compute unit");
     if (hipError_t e = allow_lds((const void*) scaled_gemm_few_kernel<OPS, NT, XR, WAVES, D, ALIGNED>, lds)) return e;
-    const dim3 grid((unsigned) ((a.N + 16 * NT - 1) / (16 * NT)), (unsigned) (a.batch[0] * a.batch[1] * a.batch[2]));
+    const dim3 grid((unsigned) (((a.M + XR - 1) / XR) * ((a.N + 16 * NT - 1) / (16 * NT))), (unsigned) (a.batch[0] * a.batch[1] * a.batch[2]));
     hipLaunchKernelGGL((scaled_gemm_few_kernel<OPS, NT, XR, WAVES, D, ALIGNED>), grid, dim3(WAVES * 64), lds, s, a);
     return hipGetLastError();
 }
@@ -200,17 +200,6 @@ hipError_t start_shaped(const ScaledGemmArgs& a, hipStream_t s)
     return a.tile_n == 1 ? start<OPS, 1, 32, 8, 3, true>(a, s) : a.tile_n == 2 ? start<OPS, 2, 32, 4, 5, true>(a, s) : start<OPS, 4, 32, 4, 3, true>(a, s);
 }
 } // namespace
-
-void scaled_gemm_few_shape(ScaledGemmArgs& a, int num_cus)
-{
-    a.tile_m = a.M <= 8 ? 8 : a.M <= 16 ? 16 : 32;
-    const long long tiles = (long long) ((a.N + 15) / 16) * a.batch[0] * a.batch[1] * a.batch[2];
-    // Fewer, larger workgroups where there are more 16-row tiles than compute units (the rings fill a unit's LDS, so one workgroup runs
-    // there at a time and a second round starts from cold): 14336 x 4096 in us with 16 / 32 / 64 rows per workgroup: one token 17.7 / 14.7 /
-    // 11.9, sixteen 20.1 / 15.8 / 12.5; 4096 x 14336: 10.9 / 11.6 / 14.2 and 11.9 / 12.7 / 16.5.
-    a.tile_n = !a.aligned || tiles <= num_cus ? 1 : tiles <= 2 * num_cus ? 2 : 4;
-    a.waves = a.tile_n == 4 || (a.tile_n == 2 && a.tile_m == 32) ? 4 : 8;
-}
 
 hipError_t launch_scaled_gemm_few(const ScaledGemmArgs& a, hipStream_t s)
 {

@@ -80,22 +80,21 @@ struct ScaledGemmArgs
     int            form;    // SCALED_FORM_*, filled in by plan_scaled_gemm
     int            tile_m, tile_n; // shape of a workgroup's outputs, in the form's own units
     int            waves;   // wavefronts per workgroup
-    int            split_k; // slices of the reduction, 1: none
-    void*          partial; // split_k > 1: split_k x batch x M x N sums (int32 / fp32)
 };
 
 enum : int
 {
-    SCALED_FORM_GENERAL = 0,
-    SCALED_FORM_FEW = 1 // few rows of x (scaled_gemm_few.hip)
+    SCALED_FORM_FEW = 0,  // few rows of x, or few outputs (scaled_gemm_few.hip): tile_m rows of x x 16 tile_n rows of w
+    SCALED_FORM_TILE = 1, // 64 x 64 or 128 x 128 outputs (scaled_gemm_tile.hip)
+    SCALED_FORM_LARGE = 2 // 256 x 256 (scaled_gemm_large.hip)
 };
 
-// picks the kernel form and the slices of the reduction for these operands; figures: what mme_hip_last_contraction_form reports
-void       plan_scaled_gemm(ScaledGemmArgs& a, int num_cus, int (&figures)[4]);
-size_t     scaled_gemm_partial_bytes(const ScaledGemmArgs& a);
+// picks the kernel form for these operands; figures: what mme_hip_last_contraction_form reports
+void plan_scaled_gemm(ScaledGemmArgs& a, int num_cus, int (&figures)[4]);
 // lets a kernel have `bytes` of dynamic LDS on the current device (asked for once per kernel and device)
 hipError_t allow_lds(const void* kernel, int bytes);
-void       scaled_gemm_few_shape(ScaledGemmArgs& a, int num_cus);
 hipError_t launch_scaled_gemm_few(const ScaledGemmArgs& a, hipStream_t s);
+hipError_t launch_scaled_gemm_tile(const ScaledGemmArgs& a, hipStream_t s);
+hipError_t launch_scaled_gemm_large(const ScaledGemmArgs& a, hipStream_t s);
 hipError_t launch_scaled_gemm(const ScaledGemmArgs& a, hipStream_t s);
 } // namespace mme
