@@ -74,6 +74,7 @@ class MmeSimTensor:
             self.is_device = data.is_cuda
         self.is_window = False
         self.desc = abi.make_tensor(self._ptr, self.sizes, dtype, fpBias, infNanMode, self.strides, dim)
+        self._ref, self._rows = C.byref(self.desc), self.sizes[1] * self.sizes[2] * self.sizes[3] * self.sizes[4]
 
     def window(self, offset, sizes, strides=None):
         """A tensor over part of this one's buffer: ``sizes`` elements from element ``offset`` on, with this tensor's strides
@@ -94,6 +95,7 @@ class MmeSimTensor:
         t.desc = abi.make_tensor(t._ptr, t.sizes, t.dtype, t.fpBias, t.infNanMode, t.strides, t.dim)
         for d, st in enumerate(t.strides):  # (a stride of 0 is meant here: the same row for every index)
             t.desc.strides[d] = st
+        t._ref, t._rows = C.byref(t.desc), t.sizes[1] * t.sizes[2] * t.sizes[3] * t.sizes[4]
         return t
 
     def _base(self):
@@ -329,42 +331,40 @@ class HipCalculator:
     def quantizeRows(self, out, rowScales, x, gate=None, gateOp=abi.GATE_SILU):
         """Rows of ``x`` (or of gate(``gate``) times ``x``) -> 8-bit codes in ``out`` and one fp32 scale per row
         (mme_hip_quantize_rows_dev).  ``rowScales``: a contiguous float32 torch tensor with one element per row."""
-        self._linear_tensors((out, x, gate), (rowScales,))
-        self._check(self._lib.mme_hip_quantize_rows_dev(self._h, out.desc, self._floats(rowScales, self._rows(out), "rowScales"), x.desc,
-                                                        gate.desc if gate is not None else None, gateOp))
+        self._linear((out, x, gate), (rowScales,))
+        self._check(self._lib.mme_hip_quantize_rows_dev(self._h, out._ref, self._floats(rowScales, out._rows, "rowScales"), x._ref,
+                                                        gate._ref if gate is not None else None, gateOp))
 
     def rmsNormQuantize(self, out, rowScales, x, gamma=None, residual=None, residualOut=None, eps=1e-6):
         """Root-mean-square norm of ``x`` (+ ``residual``, the sum kept in ``residualOut``) times ``gamma``, as 8-bit codes and one
         scale per row (mme_hip_rms_norm_quantize_dev)."""
-        self._linear_tensors((out, x, gamma, residual, residualOut), (rowScales,))
+        self._linear((out, x, gamma, residual, residualOut), (rowScales,))
         self._check(self._lib.mme_hip_rms_norm_quantize_dev(
-            self._h, out.desc, self._floats(rowScales, self._rows(out), "rowScales"), residualOut.desc if residualOut is not None else None, x.desc,
-            residual.desc if residual is not None else None, gamma.desc if gamma is not None else None, eps))
+            self._h, out._ref, self._floats(rowScales, out._rows, "rowScales"), residualOut._ref if residualOut is not None else None, x._ref,
+            residual._ref if residual is not None else None, gamma._ref if gamma is not None else None, eps))
 
     def scaledGemm(self, out, x, xScales, w, wScales, bias=None):
         """out = (x w^T) times a scale per row of x and per row of w, plus a bias per row of w, over int8 or fp8 codes
         (mme_hip_scaled_gemm_dev).  Scales and bias: contiguous float32 torch tensors, or None."""
-        self._linear_tensors((out, x, w), (xScales, wScales, bias))
-        self._check(self._lib.mme_hip_scaled_gemm_dev(self._h, out.desc, x.desc, self._floats(xScales, self._rows(x), "xScales"), w.desc,
-                                                      self._floats(wScales, self._rows(w), "wScales"), self._floats(bias, self._rows(w), "bias")))
+        self._linear((out, x, w), (xScales, wScales, bias))
+        self._check(self._lib.mme_hip_scaled_gemm_dev(self._h, out._ref, x._ref, self._floats(xScales, x._rows, "xScales"), w._ref,
+                                                      self._floats(wScales, w._rows, "wScales"), self._floats(bias, w._rows, "bias")))
 
-    @staticmethod
-    def _rows(t):
-        return t.sizes[1] * t.sizes[2] * t.sizes[3] * t.sizes[4]
-
+    # (every generated token makes these calls many times: what they check is kept to a microsecond)
     @staticmethod
     def _floats(t, n, name):
         if t is None:
             return None
-        if not t.is_cuda or t.element_size() != 4 or not t.is_floating_point() or not t.is_contiguous() or t.numel() < n:
+        if not t.is_cuda or t.element_size() != 4 or not t.is_floating_point() or t.numel() < n or not t.is_contiguous():
             raise MMEStackException("%s: a contiguous float32 device tensor of at least %d elements" % (name, n), abi.EINVAL)
         return t.data_ptr()
 
-    def _linear_tensors(self, tensors, arrays):
+    def _linear(self, tensors, arrays):
         for t in tensors:
             if t is not None and not t.is_device:
                 raise MMEStackException("the 8-bit linear layer needs device tensors", abi.EINVAL)
-        self._after_torch(*[t.data() for t in tensors if t is not None], *arrays)
+        if not self._caller_stream:
+            self._after_torch(*[t._keep for t in tensors if t is not None], *arrays)
 
     def _placement(self, *tensors):
         if any(t.is_window for t in tensors):
