@@ -143,33 +143,35 @@ __device__ __forceinline__ void store8(void* base, long long elem, int left, con
     }
 }
 
-// e^x to about one unit in the last place: the rounding error of x log2(e), which the hardware's 2^t would magnify by |x|, is
-// computed and put back to first order (x is clamped to where the result is neither 0 nor inf)
-__device__ __forceinline__ float exp_accurate(float x)
+// 1 / (1 + e^x) to about two units in the last place.  e^x is 2^t with t = x log2(e); the rounding of t, which the exponential would
+// magnify by |x|, is computed and put back to first order.
+__device__ __forceinline__ float logistic(float x)
 {
     constexpr float L2E = 0x1.715476p+0f, L2E_LO = 0x1.4ae0bep-26f, LN2 = 0x1.62e43p-1f;
-    x = __builtin_fminf(__builtin_fmaxf(x, -87.0f), 88.0f);
-    const float t = x * L2E;
-    const float r = __builtin_fmaf(x, L2E_LO, __builtin_fmaf(x, L2E, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return __builtin_fmaf(e * LN2, r, e);
+    const float     c = __builtin_amdgcn_fmed3f(x, -87.0f, 87.0f);
+    const float     t = c * L2E;
+    const float     r = __builtin_fmaf(c, L2E_LO, __builtin_fmaf(c, L2E, -t));
+    const float     e = __builtin_amdgcn_exp2f(t);
+    const float     y = __builtin_amdgcn_rcpf(1.0f + __builtin_fmaf(e * LN2, r, e));
+    return x > 87.0f ? 0.0f : y;
 }
+// g / (1 + e^-g), or its like with 2 sqrt(2 / pi) (g + 0.044715 g^3) in the exponent: the tanh form of gelu is that.  NaN gives NaN, +inf
+// gives inf and -inf NaN (inf x 0).
 __device__ __forceinline__ float gate_of(float g, int gelu)
 {
-    // (g / (1 + e^-g) and g / (1 + e^-2c): the tanh form of gelu is g sigmoid(2 c); an inf or NaN gate gives what the
-    // formula gives in the limit, NaN for NaN, inf for +inf and NaN (0 x inf) for -inf)
-    float a = -g;
-    if (gelu) a *= 2.0f * 0.7978845608028654f * __builtin_fmaf(0.044715f * g, g, 1.0f);
-    return g / (1.0f + (a > 88.0f ? __uint_as_float(0x7F800000u) : exp_accurate(a)));
+    float x = -g;
+    if (gelu) x *= 2.0f * 0.7978845608028654f * __builtin_fmaf(0.044715f * g, g, 1.0f);
+    return g * logistic(x);
 }
 
-// sum and maximum (of bit patterns of magnitudes, whose order is the values' with NaN on top) over 64 lanes: within rows of 16
-// by data-parallel moves, across them by the two lane swaps
+// sum and maximum (of bit patterns of magnitudes, whose order is the values' with NaN on top) over groups of LANES = 16, 32 or 64 lanes:
+// within rows of 16 by data-parallel moves, across them by the two lane swaps
 template<int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t x)
 {
     return (uint32_t) __builtin_amdgcn_update_dpp(0, (int) x, CTRL, 0xF, 0xF, true);
 }
+template<int LANES>
 __device__ __forceinline__ void wave_reduce(float& sum, uint32_t& top)
 {
     auto step = [&](auto ctrl) __attribute__((always_inline))
@@ -182,65 +184,54 @@ __device__ __forceinline__ void wave_reduce(float& sum, uint32_t& top)
     step(std::integral_constant<int, 0x4E>());  // quad_perm 2, 3, 0, 1
     step(std::integral_constant<int, 0x141>()); // row_half_mirror
     step(std::integral_constant<int, 0x140>()); // row_mirror
-    auto s16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-    sum = __uint_as_float(s16[0]) + __uint_as_float(s16[1]);
-    auto t16 = __builtin_amdgcn_permlane16_swap(top, top, false, false);
-    top = max(t16[0], t16[1]);
-    auto s32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-    sum = __uint_as_float(s32[0]) + __uint_as_float(s32[1]);
-    auto t32 = __builtin_amdgcn_permlane32_swap(top, top, false, false);
-    top = max(t32[0], t32[1]);
+    if constexpr (LANES > 16)
+    {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+        sum = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+        const auto t = __builtin_amdgcn_permlane16_swap(top, top, false, false);
+        top = max(t[0], t[1]);
+    }
+    if constexpr (LANES > 32)
+    {
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+        sum = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+        const auto t = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+        top = max(t[0], t[1]);
+    }
 }
 
 constexpr uint32_t INF_BITS = 0x7F800000u, LOW_BITS = 0x1F800000u /* 2^-64 */;
 
-// T lanes per row (64: four rows per workgroup, one per wavefront; else a workgroup per row), NV steps of T x 8 elements held in
-// registers; NV 0: rows of any width, gone over again in memory for every pass.
-template<int KIND, int TYPE, int T, int NV>
-__global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(const RowQuantArgs a)
+// LANES per row: 16, 32 or 64, several rows per workgroup of 256; or 0, a workgroup per row.  Each lane holds NV times 8 elements of its
+// row in registers, at every (lanes per row x 8)-th place; NV 0: rows of any width, gone over again in memory for every pass.
+template<int KIND, int TYPE, int LANES, int NV>
+__global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void row_quant_kernel(const RowQuantArgs a)
 {
     constexpr bool NORM = KIND == ROWS_NORM || KIND == ROWS_NORM_ADD;
     constexpr bool TWO = KIND == ROWS_GATED || KIND == ROWS_NORM_ADD;
-    constexpr int  WAVES = T / 64;
-    __shared__ float    part_sum[2][WAVES > 1 ? WAVES : 1];
-    __shared__ uint32_t part_top[2][WAVES > 1 ? WAVES : 1];
-    const int      lane = T == 64 ? threadIdx.x & 63 : threadIdx.x;
-    const uint32_t row = T == 64 ? blockIdx.x * 4u + (uint32_t) __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
-    if (T == 64 && row >= a.rows) return; // (no barrier is met by these instances)
-    uint32_t i0 = row, i1 = 0, i2 = 0, i3 = 0;
-    if (a.n[0] != a.rows)
+    constexpr int  N = NV ? NV : 1;
+    __shared__ float    part_sum[2][16];
+    __shared__ uint32_t part_top[2][16];
+    const int      lane = LANES ? threadIdx.x % (LANES ? LANES : 1) : threadIdx.x, lanes = LANES ? LANES : (int) blockDim.x;
+    const uint32_t row = LANES ? blockIdx.x * (256u / (LANES ? LANES : 1)) + threadIdx.x / (LANES ? LANES : 1) : blockIdx.x;
+    const bool     live = row < a.rows; // (every lane takes part in the reductions)
+    const int      width = live ? (int) a.width : 0;
+    auto           at = [&](const long long(&st)[4], uint32_t row) __attribute__((always_inline)) -> long long
     {
-        uint32_t r = row / a.n[0];
-        i0 = row - r * a.n[0];
-        i1 = r % a.n[1];
+        if (a.n[0] == a.rows) return row * st[0];
+        uint32_t       r = row / a.n[0];
+        const uint32_t i0 = row - r * a.n[0], i1 = r % a.n[1];
         r /= a.n[1];
-        i2 = r % a.n[2];
-        i3 = r / a.n[2];
-    }
-    auto at = [&](const long long (&st)[4]) __attribute__((always_inline)) { return i0 * st[0] + i1 * st[1] + i2 * st[2] + i3 * st[3]; };
-    const long long x0 = at(a.x_stride), y0 = TWO ? at(a.second_stride) : 0;
-    const int       width = (int) a.width;
-
-    // s: what the norm squares (or x), u: what the codes stand for (elements behind the row's end are zeros in both)
-    auto load_s = [&](int e, float (&s)[VEC]) __attribute__((always_inline))
-    {
-        const int  left = width - e;
-        const auto x = load8<TYPE>(a.x, x0 + e, left);
-        if constexpr (TWO)
-        {
-            const auto y = load8<TYPE>(a.second, y0 + e, left);
-#pragma unroll
-            for (int i = 0; i < VEC; i++) s[i] = KIND == ROWS_NORM_ADD ? value<TYPE>(x, i) + value<TYPE>(y, i) : gate_of(value<TYPE>(y, i), a.gelu) * value<TYPE>(x, i);
-        }
-        else
-        {
-#pragma unroll
-            for (int i = 0; i < VEC; i++) s[i] = value<TYPE>(x, i);
-        }
+        return i0 * st[0] + i1 * st[1] + (r % a.n[2]) * st[2] + (r / a.n[2]) * st[3];
     };
-    auto load_gamma = [&](int e, float (&g)[VEC]) __attribute__((always_inline))
+    auto load_gamma = [&](int e, float(&g)[VEC]) __attribute__((always_inline))
     {
-        if (a.gamma_type == REAL_FP32)
+        if (!a.gamma)
+        {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) g[i] = 1.0f;
+        }
+        else if (a.gamma_type == REAL_FP32)
         {
             const auto q = load8<REAL_FP32>(a.gamma, e, width - e);
 #pragma unroll
@@ -253,63 +244,86 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(const RowQ
             for (int i = 0; i < VEC; i++) g[i] = value<TYPE>(q, i);
         }
     };
-
-    float s[NV ? NV : 1][VEC], u[NV ? NV : 1][VEC];
-    // fills u of step n; fs, fu: powers of two that the squares' operands and u are multiplied by (1 but for rows gone over again)
-    auto fill = [&](int n, int e, float fs, float fu, float& sum, uint32_t& top) __attribute__((always_inline))
+    // s: what the norm squares, or what the codes stand for (elements behind the row's end are zeros)
+    auto make_s = [&](const Raw<TYPE>& x, const Raw<TYPE>& y, float(&s)[VEC]) __attribute__((always_inline))
     {
-        if constexpr (NORM)
+#pragma unroll
+        for (int i = 0; i < VEC; i++)
+            s[i] = KIND == ROWS_NORM_ADD ? value<TYPE>(x, i) + value<TYPE>(y, i) : KIND == ROWS_GATED ? gate_of(value<TYPE>(y, i), a.gelu) * value<TYPE>(x, i) : value<TYPE>(x, i);
+    };
+    // u: what the codes stand for up to a factor of the row; fu: a power of two it is multiplied by (1 but for rows gone over again)
+    auto make_u = [&](const float(&s)[VEC], const float(&g)[VEC], float fu, float(&u)[VEC]) __attribute__((always_inline))
+    {
+        if (fu == 1.0f)
         {
-            float g[VEC];
-            if (a.gamma) load_gamma(e, g);
-            else
+#pragma unroll
+            for (int i = 0; i < VEC; i++) u[i] = NORM ? s[i] * g[i] : s[i];
+        }
+        else if (NORM)
+        {
+            // the power goes to the factor that it takes towards one: nothing overflows or vanishes on the way
+#pragma unroll
+            for (int i = 0; i < VEC; i++)
             {
-#pragma unroll
-                for (int i = 0; i < VEC; i++) g[i] = 1.0f;
+                const bool small = __builtin_fabsf(s[i]) < 1.0f, to_s = small == (fu > 1.0f);
+                u[i] = (to_s ? s[i] * fu : s[i]) * (to_s ? g[i] : g[i] * fu);
             }
-            if (fu == 1.0f)
-            {
-#pragma unroll
-                for (int i = 0; i < VEC; i++) u[n][i] = s[n][i] * g[i];
-            }
-            else
-            {
-                // the power goes to the factor that it takes towards one: nothing overflows or vanishes on the way
-#pragma unroll
-                for (int i = 0; i < VEC; i++)
-                {
-                    const bool small = __builtin_fabsf(s[n][i]) < 1.0f, to_s = small == (fu > 1.0f);
-                    u[n][i] = (to_s ? s[n][i] * fu : s[n][i]) * (to_s ? g[i] : g[i] * fu);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < VEC; i++) sum = __builtin_fmaf(s[n][i] * fs, s[n][i] * fs, sum);
         }
         else
         {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) u[n][i] = s[n][i] * fu;
+            for (int i = 0; i < VEC; i++) u[i] = s[i] * fu;
+        }
+    };
+    auto gather = [&](const float(&s)[VEC], const float(&g)[VEC], float fs, float fu, float& sum, uint32_t& top) __attribute__((always_inline))
+    {
+        float u[VEC];
+        make_u(s, g, fu, u);
+        if constexpr (NORM)
+        {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) sum = __builtin_fmaf(s[i] * fs, s[i] * fs, sum);
         }
 #pragma unroll
-        for (int i = 0; i < VEC; i++) top = max(top, __float_as_uint(u[n][i]) & 0x7FFFFFFFu);
+        for (int i = 0; i < VEC; i++) top = max(top, __float_as_uint(u[i]) & 0x7FFFFFFFu);
     };
     int  phase = 0;
     auto reduce = [&](float& sum, uint32_t& top) __attribute__((always_inline))
     {
-        wave_reduce(sum, top);
-        if constexpr (WAVES > 1)
+        wave_reduce<LANES ? LANES : 64>(sum, top);
+        if constexpr (LANES == 0)
         {
-            // (two sets of cells used in turn: a second reduction does not overwrite what a slow wavefront still reads)
-            const int wave = threadIdx.x >> 6;
+            // (two sets of cells used in turn: the second reduction does not overwrite what a slow wavefront still reads of the first)
+            const int wave = threadIdx.x >> 6, w = threadIdx.x & 15, waves = (int) blockDim.x >> 6;
             if ((threadIdx.x & 63) == 0) part_sum[phase][wave] = sum, part_top[phase][wave] = top;
             __syncthreads();
-            const int w = threadIdx.x & 63;
-            sum = w < WAVES ? part_sum[phase][w] : 0.0f;
-            top = w < WAVES ? part_top[phase][w] : 0u;
-            wave_reduce(sum, top);
+            sum = w < waves ? part_sum[phase][w] : 0.0f;
+            top = w < waves ? part_top[phase][w] : 0u;
+            wave_reduce<16>(sum, top);
             phase ^= 1;
         }
     };
+
+    float           gamma[N][VEC], s[N][VEC];
+    const long long x0 = at(a.x_stride, row), y0 = TWO ? at(a.second_stride, row) : 0, c0 = at(a.codes_stride, row), r0 = KIND == ROWS_NORM_ADD ? at(a.sum_stride, row) : 0;
+    if constexpr (NV > 0)
+    {
+        Raw<TYPE> x[N], y[N];
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+        {
+            const int e = (n * lanes + lane) * VEC;
+            x[n] = load8<TYPE>(a.x, x0 + e, width - e);
+            if constexpr (TWO) y[n] = load8<TYPE>(a.second, y0 + e, width - e);
+        }
+        if constexpr (NORM)
+        {
+#pragma unroll
+            for (int n = 0; n < NV; n++) load_gamma((n * lanes + lane) * VEC, gamma[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < NV; n++) make_s(x[n], y[n], s[n]);
+    }
     auto pass = [&](float fs, float fu, float& sum, uint32_t& top) __attribute__((always_inline))
     {
         sum = 0.0f;
@@ -317,64 +331,50 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(const RowQ
         if constexpr (NV > 0)
         {
 #pragma unroll
-            for (int n = 0; n < NV; n++) fill(n, (n * T + lane) * VEC, fs, fu, sum, top);
+            for (int n = 0; n < NV; n++) gather(s[n], gamma[n], fs, fu, sum, top);
         }
         else
         {
 #pragma unroll 1
-            for (int e = lane * VEC; e < width; e += T * VEC)
+            for (int e = lane * VEC; e < width; e += lanes * VEC)
             {
-                load_s(e, s[0]);
-                fill(0, e, fs, fu, sum, top);
+                const auto xe = load8<TYPE>(a.x, x0 + e, width - e);
+                Raw<TYPE>  ye = xe;
+                if constexpr (TWO) ye = load8<TYPE>(a.second, y0 + e, width - e);
+                make_s(xe, ye, s[0]);
+                if constexpr (NORM) load_gamma(e, gamma[0]);
+                gather(s[0], gamma[0], fs, fu, sum, top);
             }
         }
         reduce(sum, top);
     };
-
-    if constexpr (NV > 0)
-    {
-#pragma unroll
-        for (int n = 0; n < NV; n++)
-        {
-            const int e = (n * T + lane) * VEC;
-            if (e < width) load_s(e, s[n]);
-            else
-            {
-#pragma unroll
-                for (int i = 0; i < VEC; i++) s[n][i] = 0.0f;
-            }
-        }
-    }
     float    fs = 1.0f, fu = 1.0f, sum;
     uint32_t top;
-    pass(fs, fu, sum, top);
-    if (top >= INF_BITS || top < LOW_BITS || (NORM && !(sum < 0x1p+126f && sum > 0x1p-100f)))
+    pass(1.0f, 1.0f, sum, top);
+    const bool odd = top >= INF_BITS || top < LOW_BITS || (NORM && !(sum < 0x1p+126f && sum > 0x1p-100f)); // (the same in every lane of the row)
+    if (LANES ? __any(odd && live) : odd)
     {
-        // (the same in every lane of the row)
+        // (a wavefront with several rows goes over all of them, those that need it not with factors of one)
         fu = top >= INF_BITS ? 0x1p-96f : (top < LOW_BITS ? 0x1p+96f : 1.0f);
         if (NORM) fs = !(sum < 0x1p+126f) ? 0x1p-96f : (sum > 0x1p-100f ? 1.0f : 0x1p+96f);
         pass(fs, fu, sum, top);
     }
-    // an inf or NaN among s shows in the squares' sum as well as in u unless gamma is zero there
     const bool  bad = top >= INF_BITS || (NORM && !(sum < __uint_as_float(INF_BITS)));
     const float most = __uint_as_float(top);
     // qmax / max|u| in two parts, f the quotient rounded to fp32, f_lo what that leaves out
     const float f = bad || top == 0u ? 0.0f : a.qmax / most;
     const float f_lo = bad || top == 0u ? 0.0f : __builtin_fmaf(-f, most, a.qmax) / most;
 
-    const long long c0 = at(a.codes_stride);
-    auto            put = [&](int n, int e) __attribute__((always_inline))
+    auto put = [&](int n, int e) __attribute__((always_inline))
     {
         const int left = width - e;
         if constexpr (KIND == ROWS_NORM_ADD)
-            if (a.sum) store8<TYPE>(a.sum, at(a.sum_stride) + e, left, rounded<TYPE>(s[n]));
+            if (a.sum) store8<TYPE>(a.sum, r0 + e, left, rounded<TYPE>(s[n]));
         uint32_t c[2] = {0u, 0u};
         if (!bad)
         {
-            float q[VEC];
-            if (a.code != CODE_INT8)
-#pragma unroll
-                for (int i = 0; i < VEC; i++) q[i] = __builtin_amdgcn_fmed3f(__builtin_fmaf(u[n][i], f, u[n][i] * f_lo), -a.qmax, a.qmax);
+            float u[VEC];
+            make_u(s[n], gamma[n], fu, u);
             if (a.code == CODE_INT8)
             {
                 // added to 1.5 x 2^23 the product is rounded once, to a whole number (127 for the largest: f is off by less than
@@ -384,29 +384,34 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(const RowQ
                 {
                     uint32_t b[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) b[i] = __float_as_uint(__builtin_fmaf(u[n][4 * h + i], f, 12582912.0f));
+                    for (int i = 0; i < 4; i++) b[i] = __float_as_uint(__builtin_fmaf(u[4 * h + i], f, 12582912.0f));
                     const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x04000C0Cu);
                     c[h] = lo | hi;
-                }
-            }
-            else if (a.code == CODE_E4M3)
-            {
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                {
-                    int p = 0;
-                    p = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h], q[4 * h + 1], p, false);
-                    c[h] = (uint32_t) __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * h + 2], q[4 * h + 3], p, true);
                 }
             }
             else
             {
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int i = 0; i < VEC; i++) u[i] = __builtin_amdgcn_fmed3f(__builtin_fmaf(u[i], f, u[i] * f_lo), -a.qmax, a.qmax);
+                if (a.code == CODE_E4M3)
                 {
-                    int p = 0;
-                    p = __builtin_amdgcn_cvt_pk_bf8_f32(q[4 * h], q[4 * h + 1], p, false);
-                    c[h] = (uint32_t) __builtin_amdgcn_cvt_pk_bf8_f32(q[4 * h + 2], q[4 * h + 3], p, true);
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                    {
+                        int p = 0;
+                        p = __builtin_amdgcn_cvt_pk_fp8_f32(u[4 * h], u[4 * h + 1], p, false);
+                        c[h] = (uint32_t) __builtin_amdgcn_cvt_pk_fp8_f32(u[4 * h + 2], u[4 * h + 3], p, true);
+                    }
+                }
+                else
+                {
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                    {
+                        int p = 0;
+                        p = __builtin_amdgcn_cvt_pk_bf8_f32(u[4 * h], u[4 * h + 1], p, false);
+                        c[h] = (uint32_t) __builtin_amdgcn_cvt_pk_bf8_f32(u[4 * h + 2], u[4 * h + 3], p, true);
+                    }
                 }
             }
         }
@@ -424,23 +429,24 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(const RowQ
 #pragma unroll
         for (int n = 0; n < NV; n++)
         {
-            const int e = (n * T + lane) * VEC;
+            const int e = (n * lanes + lane) * VEC;
             if (e < width) put(n, e);
         }
     }
     else
     {
 #pragma unroll 1
-        for (int e = lane * VEC; e < width; e += T * VEC)
+        for (int e = lane * VEC; e < width; e += lanes * VEC)
         {
-            float    dummy_sum = 0.0f;
-            uint32_t dummy_top = 0u;
-            load_s(e, s[0]);
-            fill(0, e, fs, fu, dummy_sum, dummy_top);
+            const auto xe = load8<TYPE>(a.x, x0 + e, width - e);
+            Raw<TYPE>  ye = xe;
+            if constexpr (TWO) ye = load8<TYPE>(a.second, y0 + e, width - e);
+            make_s(xe, ye, s[0]);
+            if constexpr (NORM) load_gamma(e, gamma[0]);
             put(0, e);
         }
     }
-    if (lane == 0)
+    if (lane == 0 && live)
     {
         double sc = (double) most / (double) a.qmax * a.fold / (double) fu;
         if (NORM)
@@ -452,24 +458,33 @@ __global__ __launch_bounds__(T == 64 ? 256 : T) void row_quant_kernel(const RowQ
     }
 }
 
-template<int KIND, int TYPE, int T, int NV>
-hipError_t start(const RowQuantArgs& a, hipStream_t s)
+template<int KIND, int TYPE, int LANES, int NV>
+hipError_t start(const RowQuantArgs& a, uint32_t threads, hipStream_t s)
 {
-    const uint32_t groups = T == 64 ? (a.rows + 3) / 4 : a.rows;
-    hipLaunchKernelGGL((row_quant_kernel<KIND, TYPE, T, NV>), dim3(groups), dim3(T == 64 ? 256 : T), 0, s, a);
+    const uint32_t per_group = LANES ? 256 / (LANES ? LANES : 1) : 1;
+    hipLaunchKernelGGL((row_quant_kernel<KIND, TYPE, LANES, NV>), dim3((a.rows - 1) / per_group + 1), dim3(threads), 0, s, a);
     return hipGetLastError();
 }
 
+// Lanes without elements cost the instructions of those that have some, so the number of lanes follows the width: as many wavefronts as
+// the row needs at 8, 16 or 32 elements a lane.  us (TB/s): norm with residual, bf16 -> e4m3, 8192 x 4096 with 512 lanes x 8
+// elements 43.6 (5.4), 256 x 16 46.7, 128 x 32 53.6; 16384 x 1024: 128 x 8 24.7, 64 x 16 26.9, 256 x 8 29.9; without residual, 8192 x 8192: 512 x 16
+// 45.3, 1024 x 8 61.3, 256 x 32 57.9; gated, 8192 x 14336: 448 x 32 109.9 (5.3), 1024 x 16 (an eighth of them idle) 116.9.  Rows of up to 512 share a workgroup: norm with
+// residual, 16384 x 64: 16 lanes each 5.5, 64 lanes each 10.8.  A workgroup that walks over rows, gamma in registers and the next row on its way,
+// needs too many registers: 46.9 for the first of these.
 template<int KIND, int TYPE>
 hipError_t start_sized(const RowQuantArgs& a, int num_cus, hipStream_t s)
 {
-    (void) num_cus;
-    if (a.width <= 512) return start<KIND, TYPE, 64, 1>(a, s);
-    if (a.width <= 1024) return start<KIND, TYPE, 64, 2>(a, s);
-    if (a.width <= 4096) return start<KIND, TYPE, 256, 2>(a, s);
-    if (a.width <= 8192) return start<KIND, TYPE, 512, 2>(a, s);
-    if (a.width <= 16384) return start<KIND, TYPE, 1024, 2>(a, s);
-    return start<KIND, TYPE, 1024, 0>(a, s);
+    constexpr bool NORM = KIND == ROWS_NORM || KIND == ROWS_NORM_ADD;
+    auto           threads = [&](uint32_t each) { return ((a.width + each * 64 - 1) / (each * 64)) * 64; };
+    if (a.width <= 128) return start<KIND, TYPE, 16, 1>(a, 256, s);
+    if (a.width <= 256) return start<KIND, TYPE, 32, 1>(a, 256, s);
+    if (a.width <= 512) return start<KIND, TYPE, 64, 1>(a, 256, s);
+    if (a.width <= 4096) return start<KIND, TYPE, 0, 1>(a, threads(8), s);
+    if constexpr (!NORM && TYPE != REAL_FP32) // (sums, gammas and wide inputs want the registers: fp32, gated, 2000 x 11008: 41.0, 38.3 with 16)
+        if (a.width > 8192 && a.width <= 16384 && a.rows >= (uint32_t) num_cus) return start<KIND, TYPE, 0, 4>(a, threads(32), s);
+    if (a.width <= 16384) return start<KIND, TYPE, 0, 2>(a, threads(16), s);
+    return start<KIND, TYPE, 0, 0>(a, 1024, s);
 }
 
 template<int KIND>
