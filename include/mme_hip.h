@@ -603,6 +603,17 @@ int mme_hip_scaled_gemm_dev(mme_hip_handle        h,
 int mme_hip_plan_scaled_gemm(const mme_hip_tensor* out, const mme_hip_tensor* x, const mme_hip_tensor* w, int num_cus, int fp8_specials_policy,
                              int form[4], char* error, size_t error_bytes);
 
+/*
+ * The same for the row quantisers: form[0] lanes that share a row, form[1] elements of it that each holds in registers (0: the row is
+ * gone over in memory), form[2] rows per workgroup, form[3] 1 when every tensor has one pitch for all its rows.  The addresses are
+ * compared with each other as the real call compares them (outputs may not meet inputs), so they have to be distinct.
+ */
+int mme_hip_plan_quantize_rows(const mme_hip_tensor* out, float* row_scales, const mme_hip_tensor* x, const mme_hip_tensor* gate, int gate_op, int num_cus,
+                               int form[4], char* error, size_t error_bytes);
+int mme_hip_plan_rms_norm_quantize(const mme_hip_tensor* out, float* row_scales, const mme_hip_tensor* residual_out, const mme_hip_tensor* x,
+                                   const mme_hip_tensor* residual, const mme_hip_tensor* gamma, float eps, int num_cus, int form[4], char* error,
+                                   size_t error_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -257,6 +257,27 @@ public:
         const mme_hip_tensor m = pod(memory), o = pod(mmeOut);
         check(mme_hip_memory_write_dev(m_h, &m, &o, reductionOp, reductionRm, clipFp));
     }
+    /* 8-bit linear layer (mme_hip_quantize_rows_dev, mme_hip_rms_norm_quantize_dev, mme_hip_scaled_gemm_dev; no counterpart in the
+     * reference): tensors and scales in device memory.  gate, gamma, residual and residualOut may be null. */
+    template<class T>
+    void quantizeRowsDev(T& output, float* rowScales, const T& x, const T* gate = nullptr, int gateOp = MME_HIP_GATE_SILU)
+    {
+        const mme_hip_tensor o = pod(output), v = pod(x), g = gate ? pod(*gate) : v;
+        check(mme_hip_quantize_rows_dev(m_h, &o, rowScales, &v, gate ? &g : nullptr, gateOp));
+    }
+    template<class T>
+    void rmsNormQuantizeDev(T& output, float* rowScales, const T& x, const T* gamma = nullptr, const T* residual = nullptr, T* residualOut = nullptr,
+                            float eps = 1e-6f)
+    {
+        const mme_hip_tensor o = pod(output), v = pod(x), g = gamma ? pod(*gamma) : v, r = residual ? pod(*residual) : v, s = residualOut ? pod(*residualOut) : v;
+        check(mme_hip_rms_norm_quantize_dev(m_h, &o, rowScales, residualOut ? &s : nullptr, &v, residual ? &r : nullptr, gamma ? &g : nullptr, eps));
+    }
+    template<class T>
+    void scaledGemmDev(T& output, const T& x, const float* xScales, const T& w, const float* wScales, const float* bias = nullptr)
+    {
+        const mme_hip_tensor o = pod(output), a = pod(x), b = pod(w);
+        check(mme_hip_scaled_gemm_dev(m_h, &o, &a, xScales, &b, wScales, bias));
+    }
     void* stream() const { return mme_hip_stream(m_h); }
     void  setStream(void* hipStream) { check(mme_hip_set_stream(m_h, hipStream)); }
     void  synchronize() { check(mme_hip_synchronize(m_h)); }
@@ -295,6 +316,18 @@ public:
         int                       form[4];
         char                      error[512];
         const int rc = mme_hip_plan_convolution(&o, &x, &w, &y, &p, op, epilogue, numCus, fp8SpecialsPolicy, form, error, sizeof error);
+        if (rc != MME_HIP_OK) throw MMEStackException(error, rc);
+        return Form {form[0], form[1], form[2], form[3]};
+    }
+
+    /* the same for scaledGemmDev (mme_hip_plan_scaled_gemm): largeTile 1 a tile kernel, 3 the kernel for few rows of x */
+    template<class T>
+    static Form planScaledGemm(const T& output, const T& x, const T& w, int numCus = 256, int fp8SpecialsPolicy = MME_HIP_FP8_SPECIALS_CHECK)
+    {
+        const mme_hip_tensor o = pod(output), a = pod(x), b = pod(w);
+        int                  form[4];
+        char                 error[512];
+        const int            rc = mme_hip_plan_scaled_gemm(&o, &a, &b, numCus, fp8SpecialsPolicy, form, error, sizeof error);
         if (rc != MME_HIP_OK) throw MMEStackException(error, rc);
         return Form {form[0], form[1], form[2], form[3]};
     }

@@ -166,6 +166,8 @@ def load_library():
     L.mme_hip_rms_norm_quantize_dev.argtypes = [vp, _TP, vp, _TP, _TP, _TP, _TP, C.c_float]
     L.mme_hip_scaled_gemm_dev.argtypes = [vp, _TP, _TP, vp, _TP, vp, vp]
     L.mme_hip_plan_scaled_gemm.argtypes = [_TP, _TP, _TP, C.c_int, C.c_int, C.POINTER(C.c_int), C.c_char_p, C.c_size_t]
+    L.mme_hip_plan_quantize_rows.argtypes = [_TP, vp, _TP, _TP, C.c_int, C.c_int, C.POINTER(C.c_int), C.c_char_p, C.c_size_t]
+    L.mme_hip_plan_rms_norm_quantize.argtypes = [_TP, vp, _TP, _TP, _TP, _TP, C.c_float, C.c_int, C.POINTER(C.c_int), C.c_char_p, C.c_size_t]
     _lib = L
     return L
 
@@ -202,3 +204,27 @@ def plan_scaled_gemm(out, x, w, num_cus=256, fp8_specials_policy=FP8_SPECIALS_CH
     form, err = (C.c_int * 4)(), C.create_string_buffer(512)
     rc = lib.mme_hip_plan_scaled_gemm(C.byref(out), C.byref(x), C.byref(w), num_cus, fp8_specials_policy, form, err, 512)
     return _planned(rc, form, err)
+
+
+def _planned_rows(rc, form, err):
+    if rc != 0:
+        raise ValueError("%s (status %d)" % (err.value.decode(), rc))
+    return {"lanes": form[0], "elements": form[1], "rows_per_group": form[2], "one_pitch": form[3]}
+
+
+def _opt(t):
+    return C.byref(t) if t is not None else None
+
+
+def plan_quantize_rows(out, row_scales, x, gate=None, gate_op=GATE_SILU, num_cus=256):
+    """What ``mme_hip_quantize_rows_dev`` would launch (``mme_hip_plan_quantize_rows``); raises ValueError where it would refuse."""
+    form, err = (C.c_int * 4)(), C.create_string_buffer(512)
+    rc = load_library().mme_hip_plan_quantize_rows(_opt(out), row_scales, _opt(x), _opt(gate), gate_op, num_cus, form, err, 512)
+    return _planned_rows(rc, form, err)
+
+
+def plan_rms_norm_quantize(out, row_scales, x, gamma=None, residual=None, residual_out=None, eps=1e-6, num_cus=256):
+    """The same for ``mme_hip_rms_norm_quantize_dev`` (``mme_hip_plan_rms_norm_quantize``)."""
+    form, err = (C.c_int * 4)(), C.create_string_buffer(512)
+    rc = load_library().mme_hip_plan_rms_norm_quantize(_opt(out), row_scales, _opt(residual_out), _opt(x), _opt(residual), _opt(gamma), eps, num_cus, form, err, 512)
+    return _planned_rows(rc, form, err)

@@ -55,10 +55,10 @@ def build_library(verbose=False, jobs=8, only_changed=False):
 
 def build_cpp_tests():
     """Compile the C++ programs over the calculator header (host code only, g++): the known-answer program (needs a GPU to
-    run) and the planner's (runs anywhere).  Returns the path of the first."""
+    run) and the planner's and the 8-bit linear layer's (run anywhere).  Returns the path of the first."""
     root = os.path.dirname(_HERE)
     exes = []
-    for name in ("kat_calculator", "plan_calculator"):
+    for name in ("kat_calculator", "plan_calculator", "linear8_calculator"):
         src = os.path.join(root, "tests", "cpp", name + ".cpp")
         exe = os.path.join(root, "tests", "cpp", name)
         cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O1", "-Wall", "-I" + os.path.join(root, "include"), src, "-o", exe, "-L" + CSRC,

@@ -2012,8 +2012,32 @@ int quantize_rows(mme_hip_handle h, const mme_hip_tensor* out, float* row_scales
     a.qmax = out->dtype == MME_HIP_INT8 ? 127.0f : out->dtype == MME_HIP_FP8_152 ? 57344.0f : out->inf_nan_mode == MME_HIP_FULL_INF_NAN ? 240.0f : 448.0f;
     a.fold = out->dtype == MME_HIP_INT8 ? 1.0 : pow2f((int) out->fp_bias - (out->dtype == MME_HIP_FP8_143 ? 7 : 15));
     a.eps = eps;
-    LAUNCH_TRY(h, launch_row_quant(a, h->num_cus, h->stream));
+    plan_row_quant(a, h->num_cus);
+    if (h->dry_run)
+    {
+        h->last_form[0] = (int) a.lanes, h->last_form[1] = a.steps * 8, h->last_form[2] = a.lanes_shared ? 256 / a.lanes_shared : 1, h->last_form[3] = flat;
+        return MME_HIP_OK;
+    }
+    HIP_TRY(h, launch_row_quant(a, h->stream));
     return MME_HIP_OK;
+}
+
+// a planning handle's answer (see mme_hip_plan_batch_gemm), whatever the call allocates on the host
+template<class F>
+int planned(int num_cus, int fp8_specials_policy, int form[4], char* error, size_t error_bytes, F&& call)
+{
+    if (!form) return MME_HIP_EINVAL;
+    try
+    {
+        mme_hip_calc h;
+        make_planning_handle(h, num_cus, fp8_specials_policy);
+        h.last_form[0] = -1; // (no rows or no outputs: nothing is launched)
+        return planned_form(h, call(&h), form, error, error_bytes);
+    }
+    catch (...)
+    {
+        return MME_HIP_ENOMEM;
+    }
 }
 } // namespace
 
@@ -2128,18 +2152,19 @@ int mme_hip_scaled_gemm_dev(mme_hip_handle h, const mme_hip_tensor* out, const m
 int mme_hip_plan_scaled_gemm(const mme_hip_tensor* out, const mme_hip_tensor* x, const mme_hip_tensor* w, int num_cus, int fp8_specials_policy, int form[4],
                              char* error, size_t error_bytes)
 {
-    if (!form) return MME_HIP_EINVAL;
-    try
-    {
-        mme_hip_calc h;
-        make_planning_handle(h, num_cus, fp8_specials_policy);
-        h.last_form[0] = -1;
-        return planned_form(h, mme_hip_scaled_gemm_dev(&h, out, x, nullptr, w, nullptr, nullptr), form, error, error_bytes);
-    }
-    catch (...)
-    {
-        return MME_HIP_ENOMEM;
-    }
+    return planned(num_cus, fp8_specials_policy, form, error, error_bytes, [&](mme_hip_handle h) { return mme_hip_scaled_gemm_dev(h, out, x, nullptr, w, nullptr, nullptr); });
+}
+
+int mme_hip_plan_quantize_rows(const mme_hip_tensor* out, float* row_scales, const mme_hip_tensor* x, const mme_hip_tensor* gate, int gate_op, int num_cus, int form[4],
+                               char* error, size_t error_bytes)
+{
+    return planned(num_cus, 0, form, error, error_bytes, [&](mme_hip_handle h) { return mme_hip_quantize_rows_dev(h, out, row_scales, x, gate, gate_op); });
+}
+
+int mme_hip_plan_rms_norm_quantize(const mme_hip_tensor* out, float* row_scales, const mme_hip_tensor* residual_out, const mme_hip_tensor* x,
+                                   const mme_hip_tensor* residual, const mme_hip_tensor* gamma, float eps, int num_cus, int form[4], char* error, size_t error_bytes)
+{
+    return planned(num_cus, 0, form, error, error_bytes, [&](mme_hip_handle h) { return mme_hip_rms_norm_quantize_dev(h, out, row_scales, residual_out, x, residual, gamma, eps); });
 }
 
 } // extern "C"

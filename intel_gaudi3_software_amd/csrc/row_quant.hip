@@ -466,48 +466,77 @@ hipError_t start(const RowQuantArgs& a, uint32_t threads, hipStream_t s)
     return hipGetLastError();
 }
 
+template<int KIND, int TYPE>
+hipError_t start_sized(const RowQuantArgs& a, hipStream_t s)
+{
+    constexpr bool NORM = KIND == ROWS_NORM || KIND == ROWS_NORM_ADD;
+    switch (a.lanes_shared)
+    {
+        case 16: return start<KIND, TYPE, 16, 1>(a, 256, s);
+        case 32: return start<KIND, TYPE, 32, 1>(a, 256, s);
+        case 64: return start<KIND, TYPE, 64, 1>(a, 256, s);
+        default: break;
+    }
+    if constexpr (!NORM && TYPE != REAL_FP32)
+        if (a.steps == 4) return start<KIND, TYPE, 0, 4>(a, a.lanes, s);
+    return a.steps == 1 ? start<KIND, TYPE, 0, 1>(a, a.lanes, s) : a.steps == 2 ? start<KIND, TYPE, 0, 2>(a, a.lanes, s) : start<KIND, TYPE, 0, 0>(a, a.lanes, s);
+}
+
+template<int KIND>
+hipError_t start_typed(const RowQuantArgs& a, hipStream_t s)
+{
+    switch (a.type)
+    {
+        case REAL_BF16: return start_sized<KIND, REAL_BF16>(a, s);
+        case REAL_FP16: return start_sized<KIND, REAL_FP16>(a, s);
+        default: return start_sized<KIND, REAL_FP32>(a, s);
+    }
+}
+} // namespace
+
 // Lanes without elements cost the instructions of those that have some, so the number of lanes follows the width: as many wavefronts as
 // the row needs at 8, 16 or 32 elements a lane.  us (TB/s): norm with residual, bf16 -> e4m3, 8192 x 4096 with 512 lanes x 8
 // elements 43.6 (5.4), 256 x 16 46.7, 128 x 32 53.6; 16384 x 1024: 128 x 8 24.7, 64 x 16 26.9, 256 x 8 29.9; without residual, 8192 x 8192: 512 x 16
 // 45.3, 1024 x 8 61.3, 256 x 32 57.9; gated, 8192 x 14336: 448 x 32 109.9 (5.3), 1024 x 16 (an eighth of them idle) 116.9.  Rows of up to 512 share a workgroup: norm with
 // residual, 16384 x 64: 16 lanes each 5.5, 64 lanes each 10.8.  A workgroup that walks over rows, gamma in registers and the next row on its way,
 // needs too many registers: 46.9 for the first of these.
-template<int KIND, int TYPE>
-hipError_t start_sized(const RowQuantArgs& a, int num_cus, hipStream_t s)
+void plan_row_quant(RowQuantArgs& a, int num_cus)
 {
-    constexpr bool NORM = KIND == ROWS_NORM || KIND == ROWS_NORM_ADD;
-    auto           threads = [&](uint32_t each) { return ((a.width + each * 64 - 1) / (each * 64)) * 64; };
-    if (a.width <= 128) return start<KIND, TYPE, 16, 1>(a, 256, s);
-    if (a.width <= 256) return start<KIND, TYPE, 32, 1>(a, 256, s);
-    if (a.width <= 512) return start<KIND, TYPE, 64, 1>(a, 256, s);
-    if (a.width <= 4096) return start<KIND, TYPE, 0, 1>(a, threads(8), s);
-    if constexpr (!NORM && TYPE != REAL_FP32) // (sums, gammas and wide inputs want the registers: fp32, gated, 2000 x 11008: 41.0, 38.3 with 16)
-        if (a.width > 8192 && a.width <= 16384 && a.rows >= (uint32_t) num_cus) return start<KIND, TYPE, 0, 4>(a, threads(32), s);
-    if (a.width <= 16384) return start<KIND, TYPE, 0, 2>(a, threads(16), s);
-    return start<KIND, TYPE, 0, 0>(a, 1024, s);
-}
-
-template<int KIND>
-hipError_t start_typed(const RowQuantArgs& a, int num_cus, hipStream_t s)
-{
-    switch (a.type)
+    auto lanes = [&](uint32_t steps) {
+        a.lanes_shared = 0;
+        a.steps = (int) steps;
+        a.lanes = ((a.width + steps * VEC * 64 - 1) / (steps * VEC * 64)) * 64;
+    };
+    const bool norm = a.kind == ROWS_NORM || a.kind == ROWS_NORM_ADD;
+    if (a.width <= 512)
     {
-        case REAL_BF16: return start_sized<KIND, REAL_BF16>(a, num_cus, s);
-        case REAL_FP16: return start_sized<KIND, REAL_FP16>(a, num_cus, s);
-        default: return start_sized<KIND, REAL_FP32>(a, num_cus, s);
+        a.lanes_shared = a.width <= 128 ? 16 : a.width <= 256 ? 32 : 64;
+        a.lanes = (uint32_t) a.lanes_shared;
+        a.steps = 1;
+    }
+    else if (a.width <= 4096)
+        lanes(1);
+    else if (a.width > 8192 && a.width <= 16384 && a.rows >= (uint32_t) num_cus && !norm && a.type != REAL_FP32)
+        lanes(4); // (sums, gammas and wide inputs want the registers: fp32, gated, 2000 x 11008: 41.0, 38.3 with 16)
+    else if (a.width <= 16384)
+        lanes(2);
+    else
+    {
+        a.lanes_shared = 0;
+        a.lanes = 1024;
+        a.steps = 0;
     }
 }
-} // namespace
 
-hipError_t launch_row_quant(const RowQuantArgs& a, int num_cus, hipStream_t s)
+hipError_t launch_row_quant(const RowQuantArgs& a, hipStream_t s)
 {
     if (a.rows == 0 || a.width == 0) return hipSuccess;
     switch (a.kind)
     {
-        case ROWS_PLAIN: return start_typed<ROWS_PLAIN>(a, num_cus, s);
-        case ROWS_GATED: return start_typed<ROWS_GATED>(a, num_cus, s);
-        case ROWS_NORM: return start_typed<ROWS_NORM>(a, num_cus, s);
-        default: return start_typed<ROWS_NORM_ADD>(a, num_cus, s);
+        case ROWS_PLAIN: return start_typed<ROWS_PLAIN>(a, s);
+        case ROWS_GATED: return start_typed<ROWS_GATED>(a, s);
+        case ROWS_NORM: return start_typed<ROWS_NORM>(a, s);
+        default: return start_typed<ROWS_NORM_ADD>(a, s);
     }
 }
 } // namespace mme

@@ -47,8 +47,13 @@ struct RowQuantArgs
     float       qmax;     // value of the largest code, exponent bias of the hardware's format
     double      fold;     // scales are multiplied by this power of two (another exponent bias)
     double      eps;
+    // filled in by plan_row_quant
+    uint32_t    lanes;        // lanes that share a row
+    int         lanes_shared; // 16, 32, 64: several rows share a workgroup of 256; 0: a workgroup per row
+    int         steps;        // eights of elements that a lane holds, 0: the row is gone over in memory
 };
-hipError_t launch_row_quant(const RowQuantArgs& a, int num_cus, hipStream_t s);
+void       plan_row_quant(RowQuantArgs& a, int num_cus);
+hipError_t launch_row_quant(const RowQuantArgs& a, hipStream_t s);
 
 // ---- scaled product --------------------------------------------------------------------------------------------------
 enum : int
