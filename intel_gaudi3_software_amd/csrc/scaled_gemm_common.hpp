@@ -149,39 +149,42 @@ struct __attribute__((packed, aligned(4))) f128_any
     float v[4];
 };
 
+// scales and biases of four consecutive columns n .. n + 3 (those below N)
+struct Columns
+{
+    f128_any sw, bias;
+};
+__device__ __forceinline__ Columns columns_of(const ScaledGemmArgs& a, const BatchOffsets& o, int n)
+{
+    Columns c = {{{1.0f, 1.0f, 1.0f, 1.0f}}, {{0.0f, 0.0f, 0.0f, 0.0f}}};
+    if (n + 4 <= a.N)
+    {
+        if (a.sw) c.sw = *(const f128_any*) (a.sw + o.sw + n);
+        if (a.bias) c.bias = *(const f128_any*) (a.bias + o.sw + n);
+    }
+    else
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+        {
+            const int q = min(n + i, a.N - 1);
+            if (a.sw) c.sw.v[i] = a.sw[o.sw + q];
+            if (a.bias) c.bias.v[i] = a.bias[o.sw + q];
+        }
+    }
+    return c;
+}
+
 // stores four consecutive outputs n .. n + 3 of row m (those below N), from their sums; sx: the row's scale
 template<class S>
-__device__ __forceinline__ void store_scaled4(const ScaledGemmArgs& a, const BatchOffsets& o, int m, int n, float sx, const S (&sum)[4])
+__device__ __forceinline__ void store_scaled4(const ScaledGemmArgs& a, const BatchOffsets& o, int m, int n, float sx, const Columns& c, const S (&sum)[4])
 {
     const long long e = o.out + (long long) m * a.out_ld + n;
     const bool      whole = n + 4 <= a.N;
     uint32_t        word[4];
-    if (a.out_type == SCALED_OUT_INT32)
-    {
 #pragma unroll
-        for (int i = 0; i < 4; i++) word[i] = (uint32_t) (int) sum[i];
-    }
-    else
-    {
-        f128_any sw = {{1.0f, 1.0f, 1.0f, 1.0f}}, bias = {{0.0f, 0.0f, 0.0f, 0.0f}};
-        if (whole)
-        {
-            if (a.sw) sw = *(const f128_any*) (a.sw + o.sw + n);
-            if (a.bias) bias = *(const f128_any*) (a.bias + o.sw + n);
-        }
-        else
-        {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-            {
-                const int q = min(n + i, a.N - 1);
-                if (a.sw) sw.v[i] = a.sw[o.sw + q];
-                if (a.bias) bias.v[i] = a.bias[o.sw + q];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) word[i] = __float_as_uint(scaled_value(sum[i], a.alpha, sx, sw.v[i], bias.v[i], a.bias != nullptr));
-    }
+    for (int i = 0; i < 4; i++)
+        word[i] = a.out_type == SCALED_OUT_INT32 ? (uint32_t) (int) sum[i] : __float_as_uint(scaled_value(sum[i], a.alpha, sx, c.sw.v[i], c.bias.v[i], a.bias != nullptr));
     if (a.out_type == SCALED_OUT_FP32 || a.out_type == SCALED_OUT_INT32)
     {
         uint32_t* p = (uint32_t*) a.out + e;

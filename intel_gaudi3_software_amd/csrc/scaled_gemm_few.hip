@@ -166,12 +166,13 @@ __global__ __launch_bounds__(WAVES * 64) void scaled_gemm_few_kernel(const Scale
         const int row = t / (4 * NT), group = t % (4 * NT), l = (group & 3) * 16 + (row & 15), block = (row >> 4) * NT + (group >> 2);
         const int m = m0 + row, n = n0 + group * 4;
         if (m >= a.M || n >= a.N) continue;
-        const float sx = scale_of_row(a, o, m);
-        v4          sum = *(const v4*) (part + (block * 64 + l) * 4);
+        const float   sx = scale_of_row(a, o, m);
+        const Columns c = columns_of(a, o, n);
+        v4            sum = *(const v4*) (part + (block * 64 + l) * 4);
 #pragma unroll
         for (int q = 1; q < WAVES; q++) sum += *(const v4*) (part + ((q * MT * NT + block) * 64 + l) * 4);
         const one s[4] = {sum[0], sum[1], sum[2], sum[3]};
-        store_scaled4(a, o, m, n, sx, s);
+        store_scaled4(a, o, m, n, sx, c, s);
     }
 }
 

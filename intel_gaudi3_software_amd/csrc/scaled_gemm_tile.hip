@@ -24,6 +24,7 @@ __global__ __launch_bounds__((4 + COPIERS) * 64) void scaled_gemm_tile_kernel(co
 {
     constexpr int WM = 2, WN = 2, WAVES = WM * WN, TM = WM * NI * 32, TN = WN * NJ * 32, ROWS = TM + TN;
     constexpr int STAGE = ROWS * 128, Q = ROWS / 8 / COPIERS; // requests per copying wavefront and stage: eight rows each
+    constexpr int P = ALIGNED ? 1 : 16 / Q; // stages that pass through registers at a time
     static_assert(Q * 8 * COPIERS == ROWS, "whole requests");
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     typedef typename Sums<OPS>::v16 v16;
@@ -35,7 +36,7 @@ __global__ __launch_bounds__((4 + COPIERS) * 64) void scaled_gemm_tile_kernel(co
     const int L = xcd * per + min(xcd, extra) + ((int) blockIdx.x >> 3);
     const int          m0 = (L % tiles_m) * TM, n0 = (L / tiles_m) * TN;
     const BatchOffsets o = batch_offsets(a, blockIdx.y);
-    const int nk = a.K >> 7; // whole stages
+    const int whole = a.K >> 7, nk = (a.K + 127) >> 7; // stages: whole ones, and all (codes behind a row's end are zeros)
     v16       acc[NI][NJ];
 #pragma unroll
     for (int i = 0; i < NI; i++)
@@ -49,56 +50,81 @@ __global__ __launch_bounds__((4 + COPIERS) * 64) void scaled_gemm_tile_kernel(co
         const int      copier = wave - WAVES, row8 = lane >> 3;
         const uint32_t lds_off = (uint32_t) (uintptr_t) lds;
         const uint8_t* src[Q];
+        int            c16[Q]; // where this lane's chunk lies in a row of the stage
 #pragma unroll
         for (int q = 0; q < Q; q++)
         {
             const int r = (q * COPIERS + copier) * 8 + row8; // row of the stage: x first
-            src[q] = (r < TM ? a.x + o.x + (long long) min(m0 + r, a.M - 1) * a.x_ld : a.w + o.w + (long long) min(n0 + r - TM, a.N - 1) * a.w_ld) +
-                     ((lane & 7) ^ swizzle(r)) * 16;
+            c16[q] = ((lane & 7) ^ swizzle(r)) * 16;
+            src[q] = r < TM ? a.x + o.x + (long long) min(m0 + r, a.M - 1) * a.x_ld : a.w + o.w + (long long) min(n0 + r - TM, a.N - 1) * a.w_ld;
         }
-        if constexpr (ALIGNED)
+        s_v4i held[P][Q]; // stages on their way through registers: all of them, or, where copies are direct, a last one that K cuts off
+        auto  load = [&](int t, int d) __attribute__((always_inline))
         {
-            // (requests beyond the last stage ask for the last one again: the number in flight is always the same)
-            auto issue = [&](int t, int slot) __attribute__((always_inline))
+            if (t < whole)
             {
 #pragma unroll
-                for (int q = 0; q < Q; q++) dma16(src[q] + (size_t) min(t, nk - 1) * 128, lds_off + slot * STAGE + (q * COPIERS + copier) * 1024);
+                for (int q = 0; q < Q; q++)
+                {
+                    const u128_any u = *(const u128_any*) (src[q] + (size_t) t * 128 + c16[q]);
+                    held[d][q] = s_v4i {(int) u.v[0], (int) u.v[1], (int) u.v[2], (int) u.v[3]};
+                }
+            }
+            else
+            {
+#pragma unroll
+                for (int q = 0; q < Q; q++) held[d][q] = load16(src[q], t * 128 + c16[q], a.K);
+            }
+        };
+        auto put = [&](int slot, int d) __attribute__((always_inline))
+        {
+#pragma unroll
+            for (int q = 0; q < Q; q++) *(s_v4i*) (lds + slot * STAGE + (q * COPIERS + copier) * 1024 + lane * 16) = held[d][q];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        };
+        if constexpr (ALIGNED)
+        {
+            auto issue = [&](int t, int slot) __attribute__((always_inline))
+            {
+                if (t < whole)
+                {
+#pragma unroll
+                    for (int q = 0; q < Q; q++) dma16(src[q] + (size_t) t * 128 + c16[q], lds_off + slot * STAGE + (q * COPIERS + copier) * 1024);
+                }
+                else if (t < nk)
+                {
+                    load(t, 0);
+                    put(slot, 0);
+                }
+            };
+            // stage t has landed once at most the requests of the whole stages behind it, up to `last`, are outstanding
+            auto landed = [&](int t, int last) __attribute__((always_inline))
+            {
+                const int behind = min(last, whole - 1) - t;
+                if (NST > 3 && behind >= 3) __builtin_amdgcn_s_waitcnt(vm_wait(3 * Q));
+                else if (NST > 2 && behind >= 2)
+                    __builtin_amdgcn_s_waitcnt(vm_wait(2 * Q));
+                else if (behind >= 1)
+                    __builtin_amdgcn_s_waitcnt(vm_wait(Q));
+                else
+                    __builtin_amdgcn_s_waitcnt(vm_wait(0));
             };
 #pragma unroll
             for (int t = 0; t < NST; t++) issue(t, t);
-            __builtin_amdgcn_s_waitcnt(vm_wait((NST - 1) * Q)); // stage 0 has landed
+            landed(0, NST - 1);
             __builtin_amdgcn_s_barrier();
             int slot = 0;
 #pragma unroll 1
             for (int t = 0; t < nk; t++)
             {
-                __builtin_amdgcn_s_waitcnt(vm_wait((NST - 2) * Q)); // stage t + 1 has landed
-                __builtin_amdgcn_s_barrier();                       // and the rest of stage t is in the others' registers: its slot is free
+                landed(t + 1, t + NST - 1);
+                __builtin_amdgcn_s_barrier(); // and the rest of stage t is in the others' registers: its slot is free
                 issue(t + NST, slot);
                 slot = slot + 1 == NST ? 0 : slot + 1;
             }
-            __builtin_amdgcn_s_waitcnt(vm_wait(0)); // (no request is left behind)
         }
         else
         {
-            // the same through registers, P stages of loads in flight
-            constexpr int P = 16 / Q;
-            s_v4i         held[P][Q];
-            auto          load = [&](int t, int d) __attribute__((always_inline))
-            {
-#pragma unroll
-                for (int q = 0; q < Q; q++)
-                {
-                    const u128_any u = *(const u128_any*) (src[q] + (size_t) min(t, nk - 1) * 128);
-                    held[d][q] = s_v4i {(int) u.v[0], (int) u.v[1], (int) u.v[2], (int) u.v[3]};
-                }
-            };
-            auto put = [&](int slot, int d) __attribute__((always_inline))
-            {
-#pragma unroll
-                for (int q = 0; q < Q; q++) *(s_v4i*) (lds + slot * STAGE + (q * COPIERS + copier) * 1024 + lane * 16) = held[d][q];
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            };
 #pragma unroll
             for (int d = 0; d < P; d++) load(d, d);
             put(0, 0);
@@ -165,58 +191,40 @@ __global__ __launch_bounds__((4 + COPIERS) * 64) void scaled_gemm_tile_kernel(co
             slot = next;
         }
     }
-    const int rest = nk * 128;
-    if (rest < a.K && wave < WAVES)
-    {
+    // the sums pass through LDS, half of the tile's rows at a time, so that consecutive lanes store consecutive groups of four columns
+    // of a row (the pitch puts rows that are stored together into different banks)
+    typedef typename Sums<OPS>::v4 v4;
+    constexpr int PITCH = TN + 4, HALF = TM / 2, LANES_N = TN / 4, ROWS_AT_A_TIME = (WAVES + COPIERS) * 64 / LANES_N;
+    static_assert(HALF * PITCH * 4 <= NST * STAGE, "half of the sums fit the ring");
+    one*          sums = (one*) lds;
+    const int     n = n0 + ((int) threadIdx.x % LANES_N) * 4;
+    const Columns cols = columns_of(a, o, n);
+    float         sx[TM / ROWS_AT_A_TIME];
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-        {
-            const int k = rest + s * 64 + (lane >> 5) * 32;
-            if (rest + s * 64 >= a.K) break;
-            s_v8i fx[NI];
+    for (int q = 0; q < TM / ROWS_AT_A_TIME; q++) sx[q] = scale_of_row(a, o, m0 + q * ROWS_AT_A_TIME + (int) threadIdx.x / LANES_N);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+    {
+        __syncthreads();
+        if (wave < WAVES && wm == h)
 #pragma unroll
             for (int i = 0; i < NI; i++)
-            {
-                const uint8_t* p = a.x + o.x + (long long) min(m0 + (wm * NI + i) * 32 + (lane & 31), a.M - 1) * a.x_ld;
-                fx[i] = join(load16(p, k, a.K), load16(p, k + 16, a.K));
-            }
 #pragma unroll
-            for (int j = 0; j < NJ; j++)
-            {
-                const uint8_t* p = a.w + o.w + (long long) min(n0 + (wn * NJ + j) * 32 + (lane & 31), a.N - 1) * a.w_ld;
-                const s_v8i    fw = join(load16(p, k, a.K), load16(p, k + 16, a.K));
+                for (int j = 0; j < NJ; j++)
 #pragma unroll
-                for (int i = 0; i < NI; i++) acc[i][j] = mma32<OPS>(fw, fx[i], acc[i][j]);
-            }
+                    for (int g = 0; g < 4; g++)
+                        *(v4*) (sums + (i * 32 + (lane & 31)) * PITCH + (wn * NJ + j) * 32 + 8 * g + 4 * (lane >> 5)) =
+                            v4 {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < HALF / ROWS_AT_A_TIME; q++)
+        {
+            const int row = q * ROWS_AT_A_TIME + (int) threadIdx.x / LANES_N, m = m0 + h * HALF + row;
+            if (m >= a.M || n >= a.N) continue;
+            const v4  v = *(const v4*) (sums + row * PITCH + n - n0);
+            const one s[4] = {v[0], v[1], v[2], v[3]};
+            store_scaled4(a, o, m, n, sx[h * (HALF / ROWS_AT_A_TIME) + q], cols, s);
         }
-    }
-    // the sums pass through LDS, so that consecutive lanes store consecutive groups of four columns of a row (pitch: two rows apart, the
-    // lanes of a store meet other banks)
-    typedef typename Sums<OPS>::v4 v4;
-    constexpr int PITCH = TN + 4;
-    static_assert(TM * PITCH * 4 <= NST * STAGE, "the sums fit the ring");
-    one* sums = (one*) lds;
-    __syncthreads();
-    if (wave < WAVES)
-#pragma unroll
-    for (int i = 0; i < NI; i++)
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-#pragma unroll
-            for (int g = 0; g < 4; g++)
-                *(v4*) (sums + ((wm * NI + i) * 32 + (lane & 31)) * PITCH + (wn * NJ + j) * 32 + 8 * g + 4 * (lane >> 5)) =
-                    v4 {acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-    __syncthreads();
-    constexpr int LANES_N = TN / 4, ROWS_AT_A_TIME = (WAVES + COPIERS) * 64 / LANES_N;
-    const int     n = n0 + ((int) threadIdx.x % LANES_N) * 4;
-#pragma unroll 4
-    for (int q = 0; q < TM / ROWS_AT_A_TIME; q++)
-    {
-        const int row = q * ROWS_AT_A_TIME + (int) threadIdx.x / LANES_N, m = m0 + row;
-        if (m >= a.M || n >= a.N) continue;
-        const v4 v = *(const v4*) (sums + row * PITCH + n - n0);
-        const one s[4] = {v[0], v[1], v[2], v[3]};
-        store_scaled4(a, o, m, n, scale_of_row(a, o, m), s);
     }
 }
 
