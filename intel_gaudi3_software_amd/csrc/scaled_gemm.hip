@@ -21,12 +21,15 @@ hipError_t allow_lds(const void* kernel, int bytes)
     return hipSuccess;
 }
 
-// What a form is expected to take: a fixed part, and for every round of workgroups over the compute units the bytes that one of them
-// brings into LDS, at the rate that a compute unit of that form was seen to reach.  Measured against the estimate, in us (M x N x K,
-// int8 -> bf16): few rows, 32 x 32 outputs, 64 x 4096 x 4096: 7.7 (6.6); 32 x 16, 64 x 1024 x 16384: 11.4 (12.7); 64 x 64 tiles, 128 x 14336 x 4096:
-// 17.2 (16.6), 250 x 4096 x 14336: 27.0 (26.4), 512 x 4096 x 4096: 17.5 (16.6); 128 x 128, 1024 x 4096 x 4096: 25.6 (25.5), 400 x 14336 x 4096: 44.7
-// (43.0); 256 x 256, 2048 x 4096 x 4096: 43.9 (41.0).  The estimates' order is the measured one in all of these; the runner-up took 5 %
-// (512 x 4096 x 4096 in 128 x 128 tiles: 21.6) to 112 % (64 x 1024 x 16384 in 64 x 64 tiles: 24.4) more.
+// What a form is expected to take: 3 us for the call, and for every round of workgroups over the compute units a fixed part (the first
+// operands' way, the sums' way out) and one per 1024 k.  The constants are fitted to 41 products, 64 x 14336 x 4096 to 16384 x 512 x
+// 320, in every form that takes them; the estimates' order is the measured one except where the first two are within 5 %.  Measured
+// in us (estimated), M x N x K, int8 -> bf16, the best form and the next:
+//   64 x 1024 x 16384     32 x 16 11.5 (14.8), 32 x 32 13.9        512 x 4096 x 4096     64 x 64 17.4 (19.2), 128 x 128 21.5
+//   250 x 4096 x 14336    64 x 64 27.4 (27.3), 32 x 64 36.7        600 x 8192 x 1024     64 x 64 16.6 (19.1), 256 x 256 17.9
+//   1024 x 4096 x 4096    128 x 128 25.7 (23.9), 64 x 64 32.4      400 x 14336 x 4096    256 x 256 42.2 (44.2), 128 x 128 45.1
+//   2048 x 4096 x 4096    256 x 256 44.0 (44.2), 128 x 128 51.2    8192 x 4096 x 256     256 x 256 27.0 (24.6), 128 x 128 51.4
+//   1000 x 4096 x 4097    128 x 128 35.5 (33.8), 64 x 64 60.0      4096 x 4096 x 4096    256 x 256 65.7 (65.4), 128 x 128 104.2
 void plan_scaled_gemm(ScaledGemmArgs& a, int num_cus, int (&figures)[4])
 {
     bool aligned = (uintptr_t) a.x % 16 == 0 && (uintptr_t) a.w % 16 == 0 && (a.M == 1 || a.x_ld % 16 == 0) && (a.N == 1 || a.w_ld % 16 == 0);
@@ -34,10 +37,12 @@ void plan_scaled_gemm(ScaledGemmArgs& a, int num_cus, int (&figures)[4])
     a.aligned = aligned;
     double best = 0.0;
     a.form = -1;
-    auto consider = [&](int form, int rows_m, int rows_n, int tile_n, int waves, double fixed_us, double gb_per_s) {
-        const double groups = (double) (((long long) a.M + rows_m - 1) / rows_m) * (double) (((long long) a.N + rows_n - 1) / rows_n) * a.batch[0] * a.batch[1] * a.batch[2];
-        const double rounds = __builtin_ceil(groups / num_cus);
-        const double us = fixed_us + rounds * (rows_m + rows_n) * (double) a.K / (gb_per_s * 1e3);
+    auto groups_of = [&](int rows_m, int rows_n) {
+        return (double) (((long long) a.M + rows_m - 1) / rows_m) * (double) (((long long) a.N + rows_n - 1) / rows_n) * a.batch[0] * a.batch[1] * a.batch[2];
+    };
+    auto consider = [&](int form, int rows_m, int rows_n, int tile_n, int waves, double us_per_round, double us_per_1024) {
+        const double groups = groups_of(rows_m, rows_n);
+        const double us = 3.0 + __builtin_ceil(groups / num_cus) * (us_per_round + us_per_1024 * a.K / 1024.0);
         if (a.form >= 0 && us >= best) return;
         best = us;
         a.form = form;
@@ -46,17 +51,19 @@ void plan_scaled_gemm(ScaledGemmArgs& a, int num_cus, int (&figures)[4])
         a.waves = waves;
     };
     const int few = a.M <= 8 ? 8 : a.M <= 16 ? 16 : 32;
-    consider(SCALED_FORM_FEW, few, 16, 1, 8, 3.5, 85.0);
+    consider(SCALED_FORM_FEW, few, 16, 1, 8, 2.2, aligned ? 0.6 : 1.07);
     if (aligned)
     {
-        consider(SCALED_FORM_FEW, few, 32, 2, few == 32 ? 4 : 8, 3.5, 85.0);
-        consider(SCALED_FORM_FEW, few, 64, 4, 4, 3.5, 85.0);
+        consider(SCALED_FORM_FEW, few, 32, 2, few == 32 ? 4 : 8, 2.5, 0.73);
+        consider(SCALED_FORM_FEW, few, 64, 4, 4, 3.4, 1.0);
     }
     if (a.M > 32)
     {
-        consider(SCALED_FORM_TILE, 64, 64, 64, 8, 3.5, 80.0);
-        consider(SCALED_FORM_TILE, 128, 128, 128, 8, 8.0, 60.0);
-        if (aligned && a.K >= 256) consider(SCALED_FORM_LARGE, 256, 256, 256, 8, 8.0, 64.0);
+        consider(SCALED_FORM_TILE, 64, 64, 64, 8, aligned ? 1.6 : 2.3, aligned ? 1.62 : 3.4);
+        consider(SCALED_FORM_TILE, 128, 128, 128, 8, aligned ? 5.9 : 7.8, aligned ? 3.75 : 5.7);
+        // the largest tiles: what one compute unit needs for 1024 k by itself, or what the operands' way to all of them takes
+        const double groups = groups_of(256, 256), fill = groups / (__builtin_ceil(groups / num_cus) * num_cus);
+        if (aligned && a.K >= 256) consider(SCALED_FORM_LARGE, 256, 256, 256, 8, 8.0, __builtin_fmax(8.3, 13.6 * fill));
     }
     figures[0] = a.form == SCALED_FORM_FEW ? 3 : 1;
     figures[1] = a.tile_m;
