@@ -586,7 +586,7 @@ int mme_hip_rms_norm_quantize_dev(mme_hip_handle        h,
  * The sum is rounded to fp32, multiplied by the scale of x, then by that of w (together with the addition of the bias in one
  * rounding), then rounded to nearest even into out's type; out of range becomes inf.  fp16 outputs have exponent bias 15.
  * The result is the same, bit for bit, for every call with the same operands, sizes and strides.  K = 0 gives the bias.  Up to 65535
- * batch elements.
+ * batch elements, K up to 2^30 (more: EUNSUPPORTED).
  */
 int mme_hip_scaled_gemm_dev(mme_hip_handle        h,
                             const mme_hip_tensor* out,

@@ -2095,7 +2095,7 @@ int mme_hip_scaled_gemm_dev(mme_hip_handle h, const mme_hip_tensor* out, const m
         for (int d = 0; d < 5; d++)
             if (out->sizes[d] == 0) return MME_HIP_OK;
         if (int8 && x->sizes[0] > 131071u) return fail(h, MME_HIP_EUNSUPPORTED, "int8: a reduction longer than 131071 may overflow its 32-bit sum");
-        if (x->sizes[0] >= (1u << 31)) return fail(h, MME_HIP_EINVAL, "x: more than 2^31 elements");
+        if (x->sizes[0] > (1u << 30)) return fail(h, MME_HIP_EUNSUPPORTED, "a reduction longer than 2^30 (the kernels look ahead of it with 32-bit indexes)");
         const uint64_t batch = (uint64_t) out->sizes[2] * out->sizes[3] * out->sizes[4];
         if (batch > 65535u) return fail(h, MME_HIP_EUNSUPPORTED, "more than 65535 batch elements");
         const uint64_t x_rows = (uint64_t) x->sizes[1] * x->sizes[2] * x->sizes[3] * x->sizes[4], w_rows = (uint64_t) w->sizes[1] * w->sizes[2] * w->sizes[3] * w->sizes[4];

@@ -25,11 +25,11 @@ hipError_t allow_lds(const void* kernel, int bytes)
 // operands' way, the sums' way out) and one per 1024 k.  The constants are fitted to 41 products, 64 x 14336 x 4096 to 16384 x 512 x
 // 320, in every form that takes them; the estimates' order is the measured one except where the first two are within 5 %.  Measured
 // in us (estimated), M x N x K, int8 -> bf16, the best form and the next:
-//   64 x 1024 x 16384     32 x 16 11.5 (14.8), 32 x 32 13.9        512 x 4096 x 4096     64 x 64 17.4 (19.2), 128 x 128 21.5
-//   250 x 4096 x 14336    64 x 64 27.4 (27.3), 32 x 64 36.7        600 x 8192 x 1024     64 x 64 16.6 (19.1), 256 x 256 17.9
-//   1024 x 4096 x 4096    128 x 128 25.7 (23.9), 64 x 64 32.4      400 x 14336 x 4096    256 x 256 42.2 (44.2), 128 x 128 45.1
-//   2048 x 4096 x 4096    256 x 256 44.0 (44.2), 128 x 128 51.2    8192 x 4096 x 256     256 x 256 27.0 (24.6), 128 x 128 51.4
-//   1000 x 4096 x 4097    128 x 128 35.5 (33.8), 64 x 64 60.0      4096 x 4096 x 4096    256 x 256 65.7 (65.4), 128 x 128 104.2
+//   64 x 1024 x 16384     32 x 16 11.5 (14.8), 32 x 32 13.9        512 x 4096 x 4096     64 x 64 16.6 (18.6), 128 x 128 21.5
+//   250 x 4096 x 14336    64 x 64 26.3 (26.3), 32 x 64 36.7        600 x 8192 x 1024     64 x 64 16.0 (18.8), 256 x 256 17.7
+//   1024 x 4096 x 4096    128 x 128 24.0 (23.6), 64 x 64 31.2      400 x 14336 x 4096    256 x 256 42.1 (44.0), 128 x 128 42.7
+//   2048 x 4096 x 4096    256 x 256 43.9 (44.0), 128 x 128 49.4    8192 x 4096 x 256     256 x 256 26.1 (24.2), 128 x 128 50.3
+//   1000 x 4096 x 4097    128 x 128 35.5 (33.0), 64 x 64 61.3      4096 x 4096 x 4096    256 x 256 64.7 (65.2), 128 x 128 103.8
 void plan_scaled_gemm(ScaledGemmArgs& a, int num_cus, int (&figures)[4])
 {
     bool aligned = (uintptr_t) a.x % 16 == 0 && (uintptr_t) a.w % 16 == 0 && (a.M == 1 || a.x_ld % 16 == 0) && (a.N == 1 || a.w_ld % 16 == 0);
@@ -59,11 +59,11 @@ void plan_scaled_gemm(ScaledGemmArgs& a, int num_cus, int (&figures)[4])
     }
     if (a.M > 32)
     {
-        consider(SCALED_FORM_TILE, 64, 64, 64, 8, aligned ? 1.6 : 2.3, aligned ? 1.62 : 3.4);
-        consider(SCALED_FORM_TILE, 128, 128, 128, 8, aligned ? 5.9 : 7.8, aligned ? 3.75 : 5.7);
+        consider(SCALED_FORM_TILE, 64, 64, 64, 8, aligned ? 1.6 : 1.8, aligned ? 1.55 : 3.4);
+        consider(SCALED_FORM_TILE, 128, 128, 128, 8, aligned ? 5.6 : 6.0, aligned ? 3.75 : 6.0);
         // the largest tiles: what one compute unit needs for 1024 k by itself, or what the operands' way to all of them takes
         const double groups = groups_of(256, 256), fill = groups / (__builtin_ceil(groups / num_cus) * num_cus);
-        if (aligned && a.K >= 256) consider(SCALED_FORM_LARGE, 256, 256, 256, 8, 8.0, __builtin_fmax(8.3, 13.6 * fill));
+        if (aligned && a.K >= 256) consider(SCALED_FORM_LARGE, 256, 256, 256, 8, 7.8, __builtin_fmax(8.3, 13.6 * fill));
     }
     figures[0] = a.form == SCALED_FORM_FEW ? 3 : 1;
     figures[1] = a.tile_m;

@@ -65,6 +65,15 @@ struct __attribute__((packed, aligned(1))) u128_any
     uint32_t v[4];
 };
 
+// sixteen codes moved down by n of them, zeros after them (none move for n <= 0, none stay for n >= 16)
+__device__ __forceinline__ s_v4i moved_down(s_v4i v, int n)
+{
+    const int          bits = 8 * min(max(n, 0), 16);
+    unsigned long long lo = ((unsigned long long) (uint32_t) v.y << 32) | (uint32_t) v.x, hi = ((unsigned long long) (uint32_t) v.w << 32) | (uint32_t) v.z;
+    lo = bits >= 128 ? 0ull : bits >= 64 ? hi >> (bits & 63) : bits ? (lo >> bits) | (hi << (64 - bits)) : lo;
+    hi = bits >= 64 ? 0ull : hi >> bits;
+    return s_v4i {(int) (uint32_t) lo, (int) (uint32_t) (lo >> 32), (int) (uint32_t) hi, (int) (uint32_t) (hi >> 32)};
+}
 // 16 codes of a row from k on, at any alignment, zeros behind the row's end
 __device__ __forceinline__ s_v4i load16(const uint8_t* row, int k, int K)
 {
@@ -77,12 +86,8 @@ __device__ __forceinline__ s_v4i load16(const uint8_t* row, int k, int K)
     if (K >= 16)
     {
         // the row's last sixteen codes, moved down by those that come before k
-        const u128_any     u = *(const u128_any*) (row + K - 16);
-        const int          bits = 8 * (k + 16 - K); // 8 .. 120
-        unsigned long long lo = ((unsigned long long) u.v[1] << 32) | u.v[0], hi = ((unsigned long long) u.v[3] << 32) | u.v[2];
-        lo = bits >= 64 ? hi >> (bits & 63) : (lo >> bits) | (hi << (64 - bits));
-        hi = bits >= 64 ? 0ull : hi >> bits;
-        return s_v4i {(int) (uint32_t) lo, (int) (uint32_t) (lo >> 32), (int) (uint32_t) hi, (int) (uint32_t) (hi >> 32)};
+        const u128_any u = *(const u128_any*) (row + K - 16);
+        return moved_down(s_v4i {(int) u.v[0], (int) u.v[1], (int) u.v[2], (int) u.v[3]}, k + 16 - K);
     }
     uint32_t v[4] = {0u, 0u, 0u, 0u};
 #pragma unroll

@@ -8,7 +8,8 @@
 // A stage is 128 k of every row of the tile, eight neighbouring lanes on a line (chunk c of row r lies at position c ^ (r / 2 & 7)); NST
 // stages form a ring.  A stage is multiplied in two halves, each while the fragments of the next are read; one barrier per stage, in its
 // middle: behind it the next stage has landed, and everybody has the rest of this one in registers, so its slot is requested
-// again.  Where all rows are 16-byte aligned the copies go directly from memory to LDS; elsewhere they pass through registers.
+// again.  Where all rows are 16-byte aligned the copies go directly from memory to LDS; elsewhere they pass through registers, up to
+// four stages of loads ahead (1000 x 4096 x 4097 35.2 us, 1000 x 4096 x 4096 24).
 // No split of the reduction: its partial sums and second kernel cost 8 us and more, and where few tiles have a long reduction the
 // form for few rows, whose wavefronts share it out, is faster at any number of rows.
 #include "scaled_gemm_common.hpp"
@@ -24,7 +25,7 @@ __global__ __launch_bounds__((4 + COPIERS) * 64) void scaled_gemm_tile_kernel(co
 {
     constexpr int WM = 2, WN = 2, WAVES = WM * WN, TM = WM * NI * 32, TN = WN * NJ * 32, ROWS = TM + TN;
     constexpr int STAGE = ROWS * 128, Q = ROWS / 8 / COPIERS; // requests per copying wavefront and stage: eight rows each
-    constexpr int P = ALIGNED ? 1 : 16 / Q; // stages that pass through registers at a time
+    constexpr int P = 16 / Q; // stages that pass through registers at a time
     static_assert(Q * 8 * COPIERS == ROWS, "whole requests");
     extern __shared__ __attribute__((aligned(1024))) char lds[];
     typedef typename Sums<OPS>::v16 v16;
@@ -49,53 +50,40 @@ __global__ __launch_bounds__((4 + COPIERS) * 64) void scaled_gemm_tile_kernel(co
     {
         const int      copier = wave - WAVES, row8 = lane >> 3;
         const uint32_t lds_off = (uint32_t) (uintptr_t) lds;
-        const uint8_t* src[Q];
-        int            c16[Q]; // where this lane's chunk lies in a row of the stage
+        const uint8_t* src[Q]; // this lane's chunk of stage 0
+        int            c16[Q]; // where it lies in its row
 #pragma unroll
         for (int q = 0; q < Q; q++)
         {
             const int r = (q * COPIERS + copier) * 8 + row8; // row of the stage: x first
             c16[q] = ((lane & 7) ^ swizzle(r)) * 16;
-            src[q] = r < TM ? a.x + o.x + (long long) min(m0 + r, a.M - 1) * a.x_ld : a.w + o.w + (long long) min(n0 + r - TM, a.N - 1) * a.w_ld;
+            src[q] = c16[q] + (r < TM ? a.x + o.x + (long long) min(m0 + r, a.M - 1) * a.x_ld : a.w + o.w + (long long) min(n0 + r - TM, a.N - 1) * a.w_ld);
         }
-        s_v4i held[P][Q]; // stages on their way through registers: all of them, or, where copies are direct, a last one that K cuts off
-        auto  load = [&](int t, int d) __attribute__((always_inline))
+        // 16 codes of stage t on their way through registers: a chunk that crosses the row's end is loaded as the row's last sixteen
+        // codes and moved into place only when it is put into LDS, so that the loads behind it stay in flight
+        auto load = [&](int t, int q) __attribute__((always_inline))
         {
-            if (t < whole)
-            {
-#pragma unroll
-                for (int q = 0; q < Q; q++)
-                {
-                    const u128_any u = *(const u128_any*) (src[q] + (size_t) t * 128 + c16[q]);
-                    held[d][q] = s_v4i {(int) u.v[0], (int) u.v[1], (int) u.v[2], (int) u.v[3]};
-                }
-            }
-            else
-            {
-#pragma unroll
-                for (int q = 0; q < Q; q++) held[d][q] = load16(src[q], t * 128 + c16[q], a.K);
-            }
+            const u128_any u = *(const u128_any*) (src[q] + min(t * 128, a.K - 16 - c16[q]));
+            return s_v4i {(int) u.v[0], (int) u.v[1], (int) u.v[2], (int) u.v[3]};
         };
-        auto put = [&](int slot, int d) __attribute__((always_inline))
-        {
-#pragma unroll
-            for (int q = 0; q < Q; q++) *(s_v4i*) (lds + slot * STAGE + (q * COPIERS + copier) * 1024 + lane * 16) = held[d][q];
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        };
+        auto in_place = [&](s_v4i v, int t, int q) __attribute__((always_inline)) { return moved_down(v, t * 128 + c16[q] - (a.K - 16)); };
+        auto put = [&](s_v4i v, int slot, int q) __attribute__((always_inline)) { *(s_v4i*) (lds + slot * STAGE + (q * COPIERS + copier) * 1024 + lane * 16) = v; };
         if constexpr (ALIGNED)
         {
             auto issue = [&](int t, int slot) __attribute__((always_inline))
             {
-                if (t < whole)
-                {
 #pragma unroll
-                    for (int q = 0; q < Q; q++) dma16(src[q] + (size_t) t * 128 + c16[q], lds_off + slot * STAGE + (q * COPIERS + copier) * 1024);
-                }
-                else if (t < nk)
-                {
-                    load(t, 0);
-                    put(slot, 0);
-                }
+                for (int q = 0; q < Q; q++) dma16(src[q] + (size_t) t * 128, lds_off + slot * STAGE + (q * COPIERS + copier) * 1024);
+            };
+            // a last stage that K cuts off
+            auto last_stage = [&](int slot) __attribute__((always_inline))
+            {
+                s_v4i v[Q];
+#pragma unroll
+                for (int q = 0; q < Q; q++) v[q] = load(whole, q);
+#pragma unroll
+                for (int q = 0; q < Q; q++) put(in_place(v[q], whole, q), slot, q);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             };
             // stage t has landed once at most the requests of the whole stages behind it, up to `last`, are outstanding
             auto landed = [&](int t, int last) __attribute__((always_inline))
@@ -110,7 +98,9 @@ __global__ __launch_bounds__((4 + COPIERS) * 64) void scaled_gemm_tile_kernel(co
                     __builtin_amdgcn_s_waitcnt(vm_wait(0));
             };
 #pragma unroll
-            for (int t = 0; t < NST; t++) issue(t, t);
+            for (int t = 0; t < NST; t++)
+                if (t < whole) issue(t, t);
+            if (whole < NST && whole < nk) last_stage(whole);
             landed(0, NST - 1);
             __builtin_amdgcn_s_barrier();
             int slot = 0;
@@ -119,16 +109,40 @@ __global__ __launch_bounds__((4 + COPIERS) * 64) void scaled_gemm_tile_kernel(co
             {
                 landed(t + 1, t + NST - 1);
                 __builtin_amdgcn_s_barrier(); // and the rest of stage t is in the others' registers: its slot is free
-                issue(t + NST, slot);
+                if (t + NST < whole) issue(t + NST, slot);
+                else if (t + NST < nk)
+                    last_stage(slot);
                 slot = slot + 1 == NST ? 0 : slot + 1;
             }
         }
         else
         {
+            // P stages are held, a row of fewer than sixteen codes (one stage) only when it is put down
+            s_v4i      held[P][Q];
+            const bool sixteen = a.K >= 16;
+            auto       take = [&](int t, int d) __attribute__((always_inline))
+            {
 #pragma unroll
-            for (int d = 0; d < P; d++) load(d, d);
-            put(0, 0);
-            load(P, 0);
+                for (int q = 0; q < Q; q++) held[d][q] = load(t, q);
+            };
+            auto put_stage = [&](int t, int slot, int d) __attribute__((always_inline))
+            {
+                if (t == whole)
+                {
+#pragma unroll
+                    for (int q = 0; q < Q; q++) held[d][q] = sixteen ? in_place(held[d][q], t, q) : load16(src[q] - c16[q], c16[q], a.K);
+                }
+#pragma unroll
+                for (int q = 0; q < Q; q++) put(held[d][q], slot, q);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            };
+            if (sixteen)
+            {
+#pragma unroll
+                for (int d = 0; d < P; d++) take(d, d);
+            }
+            put_stage(0, 0, 0);
+            if (sixteen) take(P, 0);
             __builtin_amdgcn_s_barrier();
             int slot = 0;
             // stage t + 1 is held in set (t + 1) % P
@@ -139,8 +153,8 @@ __global__ __launch_bounds__((4 + COPIERS) * 64) void scaled_gemm_tile_kernel(co
                     if (t0 + d < nk)
                     {
                         slot = slot + 1 == NST ? 0 : slot + 1;
-                        put(slot, (d + 1) % P);
-                        load(t0 + d + 1 + P, (d + 1) % P);
+                        put_stage(t0 + d + 1, slot, (d + 1) % P);
+                        if (sixteen) take(t0 + d + 1 + P, (d + 1) % P);
                         __builtin_amdgcn_s_barrier();
                     }
         }
@@ -242,8 +256,9 @@ hipError_t start(const ScaledGemmArgs& a, hipStream_t s)
 template<int OPS>
 hipError_t start_shaped(const ScaledGemmArgs& a, hipStream_t s)
 {
-    if (a.tile_m == 64) return a.aligned ? start<OPS, 1, 1, 4, true>(a, s) : start<OPS, 1, 1, 4, false>(a, s);
-    return a.aligned ? start<OPS, 2, 2, 4, true>(a, s) : start<OPS, 2, 2, 4, false>(a, s);
+    const bool direct = a.aligned && a.K >= 16;
+    if (a.tile_m == 64) return direct ? start<OPS, 1, 1, 4, true>(a, s) : start<OPS, 1, 1, 4, false>(a, s);
+    return direct ? start<OPS, 2, 2, 4, true>(a, s) : start<OPS, 2, 2, 4, false>(a, s);
 }
 } // namespace
 

@@ -189,6 +189,9 @@ def test_refusals_of_the_product():
     refused("65535", g, T(4096, [1, 1, 65536], abi.BF16), T(1, [16, 1, 65536], abi.INT8), T(2048, [16, 1], abi.INT8))
     refused("131071", g, T(4096, [1, 1], abi.BF16), T(1, [131072, 1], abi.INT8), T(2048, [131072, 1], abi.INT8))
     assert g(T(4096, [1, 1], abi.BF16), T(1, [131071, 1], abi.INT8), T(2048, [131071, 1], abi.INT8))["large_tile"] == 3
+    long = (1 << 30) + 1
+    refused("2^30", g, T(4096, [1, 1], abi.BF16), e4(1, [long, 1]), e4(2048, [long, 1]))
+    assert g(T(4096, [1, 1], abi.BF16), e4(1, [long - 1, 1]), e4(2048, [long - 1, 1]))["large_tile"] == 3
     refused("rows overlap", g, T(4096, [8, 4], abi.BF16, strides=[1, 7]), x, w)
     refused("exponent bias", g, o, e4(1, [64, 4], bias=8), e4(2048, [64, 8]))
     for a, b in ((e4(1, [64, 4], 0), e4(2048, [64, 8])), (e4(1, [64, 4]), e5(2048, [64, 8], 1)), (e4(1, [64, 4], 1), e4(2048, [64, 8]))):
