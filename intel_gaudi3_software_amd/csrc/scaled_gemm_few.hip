@@ -5,10 +5,11 @@
 //
 // The 16 x 16 matrix instructions want neighbouring lanes on neighbouring rows.  Loaded that way from memory every lane is a line
 // of its own and a compute unit takes in 17 bytes a clock; so a wavefront brings a stage (128 k of every row) into a ring of its
-// own in LDS, eight neighbouring lanes on the eight 16-byte chunks of a line, and reads it back in the instructions' layout (chunk c of
-// row r lies at position c ^ (r / 2 & 7): the sixteen rows of a read meet every bank once).  Sixteen tokens, 4096 x 14336: 11.9 us, 4.9 TB/s of w and x (loaded straight into
-// the instructions' layout: 15.2); 14336 x 4096: 12.5 us, 4.7 TB/s; one token, 4096 x 4096: 5.7 us, most of it the launch.  Where all rows are 16-byte aligned the copies are direct, memory to
-// LDS, and D stages are in flight; elsewhere they pass through registers.  The last K % 128 codes are loaded by hand.
+// own in LDS, eight neighbouring lanes on the eight 16-byte chunks of a line, and reads it back in the instructions' layout (chunk c
+// of row r lies at position c ^ (r / 2 & 7): the sixteen rows of a read meet every bank once).  Sixteen tokens, 4096 x 14336: 11.9 us,
+// 4.9 TB/s of w and x (loaded straight into the instructions' layout: 15.2); 14336 x 4096: 12.5 us, 4.7 TB/s; one token, 4096 x 4096:
+// 5.6 us, most of it the launch.  Where all rows are 16-byte aligned the copies are direct, memory to LDS, and D stages are in
+// flight; elsewhere they pass through registers.  The last K % 128 codes are loaded by hand.
 #include "scaled_gemm_common.hpp"
 
 namespace mme
