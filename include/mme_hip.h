@@ -543,7 +543,7 @@ int mme_hip_absmax_dev(mme_hip_handle h, float* out_absmax, const float* in, siz
  * row_scales: one float per row, dense in the order of the rows (dimension 1 fastest).  Arithmetic in fp32, the scale is
  * rounded once from fp64.  A row of zeros gets the scale 0 and codes of zero.  A row that holds an inf or NaN (or whose gated
  * products overflow fp32) gets the scale NaN and codes 0: NaN reaches every output of its row in the product, and no other.
- * Where the scale itself falls below 2^-126 it has fewer bits, like any denormal.
+ * Where the scale itself falls below 2^-126 it has fewer bits, like any denormal.  Up to 2^28 - 16 rows (more: EUNSUPPORTED).
  */
 int mme_hip_quantize_rows_dev(mme_hip_handle        h,
                               const mme_hip_tensor* out,
@@ -586,7 +586,7 @@ int mme_hip_rms_norm_quantize_dev(mme_hip_handle        h,
  * The sum is rounded to fp32, multiplied by the scale of x, then by that of w (together with the addition of the bias in one
  * rounding), then rounded to nearest even into out's type; out of range becomes inf.  fp16 outputs have exponent bias 15.
  * The result is the same, bit for bit, for every call with the same operands, sizes and strides.  K = 0 gives the bias.  Up to 65535
- * batch elements, K up to 2^30 (more: EUNSUPPORTED).
+ * batch elements, K up to 2^30, N up to 2^27 - 16 (more: EUNSUPPORTED).
  */
 int mme_hip_scaled_gemm_dev(mme_hip_handle        h,
                             const mme_hip_tensor* out,

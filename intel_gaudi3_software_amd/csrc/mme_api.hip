@@ -1853,6 +1853,8 @@ int linear_elem_size(int dt)
 }
 bool is_code(int dt) { return dt == MME_HIP_INT8 || is_fp8(dt); }
 
+constexpr uint64_t MOST_LANES = 0xFFFFFFFFu; // of one dimension of a launch
+
 int check_rows_tensor(mme_hip_handle h, const mme_hip_tensor* t, const char* name, bool output)
 {
     if (!t) return fail(h, MME_HIP_EINVAL, "%s: got null pointer", name);
@@ -2013,6 +2015,8 @@ int quantize_rows(mme_hip_handle h, const mme_hip_tensor* out, float* row_scales
     a.fold = out->dtype == MME_HIP_INT8 ? 1.0 : pow2f((int) out->fp_bias - (out->dtype == MME_HIP_FP8_143 ? 7 : 15));
     a.eps = eps;
     plan_row_quant(a, h->num_cus);
+    if ((uint64_t) (a.lanes_shared ? (a.rows - 1) / (256u / a.lanes_shared) + 1 : a.rows) * (a.lanes_shared ? 256u : a.lanes) > MOST_LANES)
+        return fail(h, MME_HIP_EUNSUPPORTED, "more rows than one launch takes");
     if (h->dry_run)
     {
         h->last_form[0] = (int) a.lanes, h->last_form[1] = a.steps * 8, h->last_form[2] = a.lanes_shared ? 256 / a.lanes_shared : 1, h->last_form[3] = flat;
@@ -2144,6 +2148,9 @@ int mme_hip_scaled_gemm_dev(mme_hip_handle h, const mme_hip_tensor* out, const m
         a.out_type = ot == MME_HIP_BF16 ? SCALED_OUT_BF16 : ot == MME_HIP_FP16 ? SCALED_OUT_FP16 : ot == MME_HIP_FP32 ? SCALED_OUT_FP32 : SCALED_OUT_INT32;
         a.alpha = pow2f(fold);
         plan_scaled_gemm(a, h->num_cus, h->last_form);
+        const uint64_t cols = a.form == SCALED_FORM_FEW ? 16u * a.tile_n : a.tile_n;
+        if (((uint64_t) a.M + a.tile_m - 1) / a.tile_m * (((uint64_t) a.N + cols - 1) / cols) * a.waves * 64 > MOST_LANES)
+            return fail(h, MME_HIP_EUNSUPPORTED, "more outputs than one launch takes");
         LAUNCH_TRY(h, launch_scaled_gemm(a, h->stream));
         return MME_HIP_OK;
     });

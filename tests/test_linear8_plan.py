@@ -128,6 +128,8 @@ def test_refusals_of_the_quantisers():
     assert q(T(64, [64, 0], abi.INT8), S, T(1, [64, 0], abi.FP32))["lanes"] == -1
     refused("2^31", q, T(64, [1 << 16, 1 << 15], abi.INT8), S, T(8192, [1 << 16, 1 << 15], abi.FP32))
     refused("2^31", q, T(64, [1 << 31, 1 << 31, 1 << 31, 1 << 31, 1 << 31], abi.INT8), S, x)
+    refused("one launch", q, T(8192, [1, (1 << 28) + 1], abi.INT8), 16384 * MIB, T(1, [1, (1 << 28) + 1], abi.FP32))
+    assert q(T(8192, [1, (1 << 28) - 16], abi.INT8), 16384 * MIB, T(1, [1, (1 << 28) - 16], abi.FP32))["lanes"] == 16
     refused("contiguous", q, o, S, T(1, [64, 4], abi.FP32, strides=[2, 128]))
     refused("rows overlap", q, T(64, [64, 4], abi.INT8, strides=[1, 63]), S, x)
     refused("rows overlap", q, T(64, [64, 4, 2], abi.INT8, strides=[1, 128, 63]), S, T(1, [64, 4, 2], abi.FP32))
@@ -192,6 +194,9 @@ def test_refusals_of_the_product():
     long = (1 << 30) + 1
     refused("2^30", g, T(4096, [1, 1], abi.BF16), e4(1, [long, 1]), e4(2048, [long, 1]))
     assert g(T(4096, [1, 1], abi.BF16), e4(1, [long - 1, 1]), e4(2048, [long - 1, 1]))["large_tile"] == 3
+    wide = (1 << 27) + 1
+    refused("one launch", g, T(4096, [wide, 1], abi.BF16), T(1, [1, 1], abi.INT8), T(2048, [1, wide], abi.INT8))
+    assert g(T(4096, [wide - 17, 1], abi.BF16), T(1, [1, 1], abi.INT8), T(2048, [1, wide - 17], abi.INT8))["large_tile"] == 3
     refused("rows overlap", g, T(4096, [8, 4], abi.BF16, strides=[1, 7]), x, w)
     refused("exponent bias", g, o, e4(1, [64, 4], bias=8), e4(2048, [64, 8]))
     for a, b in ((e4(1, [64, 4], 0), e4(2048, [64, 8])), (e4(1, [64, 4]), e5(2048, [64, 8], 1)), (e4(1, [64, 4], 1), e4(2048, [64, 8]))):
