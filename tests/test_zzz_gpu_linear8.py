@@ -342,6 +342,69 @@ def test_product_strided(calc, M):
     assert np.all(got[:, :, :4] == 77) and np.all(got[:, :, 4 + N:] == 77)
 
 
+@pytest.mark.parametrize("M,N,rows,aligned", [(70, 4000, 64, True), (70, 4000, 64, False), (2001, 2001, 128, True), (2001, 2001, 128, False), (4000, 4001, 256, True)])
+def test_product_tiles_at_every_kind_of_end(calc, M, N, rows, aligned):
+    """Reductions that end at every place of a stage, fewer stages than the ring holds and more, rows at even and at odd addresses."""
+    import torch
+    rng = np.random.default_rng(M)
+    seen = set()
+    for K in (1, 7, 15, 16, 17, 31, 100, 127, 128, 129, 255, 256, 272, 330, 384, 400, 511, 512, 513, 640, 645, 766, 1025):
+        x, w = _random_codes(rng, "int8", M, K), _random_codes(rng, "int8", N, K)
+        pitch, first = (-(-K // 16) * 16 + 16, 16) if aligned else (K + 3, 5)
+        tx, tw = torch.full((first + M * pitch,), 99, dtype=torch.uint8, device="cuda"), torch.full((first + N * pitch,), 99, dtype=torch.uint8, device="cuda")
+        tx[first:].view(M, pitch)[:, :K] = torch.from_numpy(x).cuda()
+        tw[first:].view(N, pitch)[:, :K] = torch.from_numpy(w).cuda()
+        out = torch.full((M, N), 77, dtype=torch.int32, device="cuda")
+        X = code_tensor(tx, [tx.numel(), 1], "int8").window(first, [K, M], [1, pitch, M * pitch, M * pitch, M * pitch])
+        W = code_tensor(tw, [tw.numel(), 1], "int8").window(first, [K, N], [1, pitch, N * pitch, N * pitch, N * pitch])
+        calc.scaledGemm(real_tensor(out, [N, M]), X, None, W, None)
+        seen.add(calc.lastContractionForm()["tile_rows"])
+        calc.synchronize()
+        value = lambda c: torch.from_numpy(c.view(np.int8)).cuda().double()
+        assert torch.equal(out.double(), value(x) @ value(w).T), K  # (exact: sums below 2^53)
+    assert rows in seen
+
+
+def test_offsets_beyond_32_bits(calc):
+    """Rows that lie further apart than 2^31 elements, of values, codes and outputs."""
+    import torch
+    rng = np.random.default_rng(8)
+    pitch, K, N = (1 << 31) + 4096, 256, 80
+    big = torch.empty(3 * pitch, dtype=torch.uint8, device="cuda")  # (6.4 GB)
+    far = lambda t, width: MmeSimTensor([big.numel() // (2 if t == abi.BF16 else 1)], 1, t, big.view(torch.bfloat16) if t == abi.BF16 else big).window(
+        0, [width, 3], [1, pitch // (2 if t == abi.BF16 else 1)] + [3 * pitch] * 3)
+    x = torch.from_numpy(rng.standard_normal((3, K))).cuda().bfloat16()
+    big.view(torch.bfloat16).view(3, pitch // 2)[:, :K] = x
+    codes, scales = torch.zeros(3, K, dtype=torch.uint8, device="cuda"), torch.zeros(3, device="cuda")
+    calc.quantizeRows(code_tensor(codes, [K, 3], "int8"), scales, far(abi.BF16, K))
+    near, near_scales = torch.zeros_like(codes), torch.zeros_like(scales)
+    calc.quantizeRows(code_tensor(near, [K, 3], "int8"), near_scales, real_tensor(x, [K, 3]))
+    calc.synchronize()
+    assert torch.equal(codes, near) and torch.equal(scales, near_scales)
+    calc.quantizeRows(far(abi.INT8, K), scales, real_tensor(x, [K, 3]))
+    w = torch.from_numpy(_random_codes(rng, "int8", N, K)).cuda()
+    out = torch.zeros(3, N, dtype=torch.bfloat16, device="cuda")
+    calc.scaledGemm(real_tensor(out, [N, 3]), far(abi.INT8, K), scales, code_tensor(w, [K, N], "int8"), None)
+    near_out = torch.zeros_like(out)
+    calc.scaledGemm(real_tensor(near_out, [N, 3]), code_tensor(near, [K, 3], "int8"), scales, code_tensor(w, [K, N], "int8"), None)
+    calc.synchronize()
+    assert torch.equal(out, near_out)
+    # the rows of w, in tiles, and the output
+    many = torch.from_numpy(_random_codes(rng, "int8", 200, K)).cuda()
+    calc.scaledGemm(far(abi.BF16, 3).window(0, [3, 3]), code_tensor(near, [K, 3], "int8"), scales, code_tensor(near, [K, 3], "int8"), None)
+    want = torch.zeros(3, 3, dtype=torch.bfloat16, device="cuda")
+    calc.scaledGemm(real_tensor(want, [3, 3]), code_tensor(near, [K, 3], "int8"), scales, code_tensor(near, [K, 3], "int8"), None)
+    calc.synchronize()
+    assert torch.equal(big.view(torch.bfloat16).view(3, pitch // 2)[:, :3], want)
+    big.view(3, pitch)[:, :K] = near
+    torch.cuda.synchronize()
+    tall, want = torch.zeros(200, 3, dtype=torch.bfloat16, device="cuda"), torch.zeros(200, 3, dtype=torch.bfloat16, device="cuda")
+    calc.scaledGemm(real_tensor(tall, [3, 200]), code_tensor(many, [K, 200], "int8"), None, far(abi.INT8, K), scales)
+    calc.scaledGemm(real_tensor(want, [3, 200]), code_tensor(many, [K, 200], "int8"), None, code_tensor(near, [K, 3], "int8"), scales)
+    calc.synchronize()
+    assert torch.equal(tall, want)
+
+
 def test_product_without_reduction_and_without_rows(calc):
     import torch
     bias = torch.tensor([1.0, -2.0, 3.0], device="cuda")
