@@ -26,6 +26,11 @@ class MMEStackException(RuntimeError):
         self.status = status
 
 
+def _descriptor_holds(sizes, strides):
+    """Whether a descriptor's unsigned 32-bit fields hold these (the stride of a single index is never used)."""
+    return all(0 <= sz < 1 << 32 and (sz <= 1 or 0 <= st < 1 << 32) for sz, st in zip(sizes, strides))
+
+
 class MmeSimTensor:
     """Descriptor + storage.  ``sizes[0]`` is the contiguous dimension (sim_tensor_base.h:52-54).
 
@@ -72,6 +77,8 @@ class MmeSimTensor:
             self._keep = data
             self._ptr = data.data_ptr()
             self.is_device = data.is_cuda
+        self._gpu = data.get_device() if self.is_device else -1
+        self._fits = _descriptor_holds(self.sizes, self.strides)
         self.is_window = False
         self.desc = abi.make_tensor(self._ptr, self.sizes, dtype, fpBias, infNanMode, self.strides, dim)
         self._ref, self._rows = C.byref(self.desc), self.sizes[1] * self.sizes[2] * self.sizes[3] * self.sizes[4]
@@ -89,6 +96,9 @@ class MmeSimTensor:
         held = self._keep.size if isinstance(self._keep, np.ndarray) else self._keep.numel()
         first = (self._ptr - self._base()) // abi.DTYPE_SIZE[self.dtype] + offset
         last = first + sum(st * (sz - 1) for st, sz in zip(t.strides, t.sizes))
+        t._gpu, t._fits = self._gpu, True
+        if not _descriptor_holds(t.sizes, t.strides):
+            raise ValueError("sizes and strides are unsigned 32-bit numbers")
         if offset < 0 or first < 0 or (min(t.sizes) > 0 and last >= held):
             raise ValueError("the window leaves the tensor's buffer")
         t._keep, t._ptr, t.is_window = self._keep, self._ptr + offset * abi.DTYPE_SIZE[self.dtype], True
@@ -177,6 +187,9 @@ class HipCalculator:
             raise MMEStackException(self._lib.mme_hip_last_error(None).decode(), rc)
         self._caller_stream = False
         self._in_flight = []   # device operands of calls since the last synchronize()
+        gpu = C.c_int()
+        self._lib.hipGetDevice(C.byref(gpu))
+        self._gpu = gpu.value  # the device that was current, which is the handle's
 
     def close(self):
         if getattr(self, "_h", None) is not None and self._h.value:
@@ -351,18 +364,19 @@ class HipCalculator:
                                                       self._floats(wScales, w._rows, "wScales"), self._floats(bias, w._rows, "bias")))
 
     # (every generated token makes these calls many times: what they check is kept to a microsecond)
-    @staticmethod
-    def _floats(t, n, name):
+    def _floats(self, t, n, name):
         if t is None:
             return None
-        if not t.is_cuda or t.element_size() != 4 or not t.is_floating_point() or t.numel() < n or not t.is_contiguous():
-            raise MMEStackException("%s: a contiguous float32 device tensor of at least %d elements" % (name, n), abi.EINVAL)
+        if t.get_device() != self._gpu or t.element_size() != 4 or not t.is_floating_point() or t.numel() < n or not t.is_contiguous():
+            raise MMEStackException("%s: a contiguous float32 tensor of at least %d elements on the calculator's device" % (name, n), abi.EINVAL)
         return t.data_ptr()
 
     def _linear(self, tensors, arrays):
         for t in tensors:
-            if t is not None and not t.is_device:
-                raise MMEStackException("the 8-bit linear layer needs device tensors", abi.EINVAL)
+            if t is not None and (t._gpu != self._gpu or not t._fits):
+                if t._fits:
+                    raise MMEStackException("the 8-bit linear layer needs device tensors, on the calculator's device", abi.EINVAL)
+                raise MMEStackException("sizes and strides are unsigned 32-bit numbers", abi.EINVAL)
         if not self._caller_stream:
             self._after_torch(*[t._keep for t in tensors if t is not None], *arrays)
 

@@ -232,3 +232,18 @@ def test_cpp_surface():
     r = subprocess.run([exe], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, timeout=60)
     text = r.stdout.decode(errors="replace")
     assert r.returncode == 0 and "all ok" in text, text
+
+
+def test_windows():
+    """Part of a buffer, inside it, with strides that a descriptor holds (on host memory: a window is a descriptor)."""
+    t = MmeSimTensor([16, 8], 2, abi.FP32)
+    w = t.window(20, [4, 3])
+    assert list(w.desc.sizes) == [4, 3, 1, 1, 1] and w.desc.strides[1] == 16 and w.desc.data == t.desc.data + 80
+    assert t.window(0, [16, 5], [1, 0]).desc.strides[1] == 0 and t.window(64, [16, 4]).window(16, [16, 3]).desc.data == t.desc.data + 320
+    assert t.window(0, [16, 1], [1, 1 << 40]).sizes[1] == 1  # (the stride of a single row is never used)
+    for offset, sizes, strides in ((0, [16, 9], None), (-1, [4, 3], None), (1, [16, 8], None), (64, [4, 3], [1, -16]), (0, [4, 2], [1, 1 << 32]), (0, [-1, 2], None),
+                                   (0, [1 << 32, 0], None)):
+        with pytest.raises(ValueError):
+            t.window(offset, sizes, strides)
+    long = MmeSimTensor([16, 8], 2, abi.FP32, np.zeros(128, np.float32), strides=[1, -16])
+    assert not long._fits and t._fits

@@ -652,6 +652,12 @@ def test_refusals(calc):
     refused(lambda: calc.doActivation(X(), X().window(0, [64, 4])), abi.EUNSUPPORTED, "windows")
     with pytest.raises(ValueError):
         X().window(1, [64, 4])
+    # a tensor of another device, sizes that a descriptor does not hold
+    away, huge = X(), X()
+    away._gpu, huge._fits = calc._gpu + 1, False
+    refused(lambda: calc.quantizeRows(C8(), sc, away), abi.EINVAL, "calculator's device")
+    refused(lambda: calc.quantizeRows(C8(), sc, huge), abi.EINVAL, "32-bit")
+    refused(lambda: calc.quantizeRows(C8(), sc.cpu(), X()), abi.EINVAL, "calculator's device")
     # (and the other entry points do not take the new types)
     refused(lambda: calc.doBatchGemm(O(), C8(), C8(8), abi.OP_ABT), abi.EINVAL, "")
     calc.synchronize()
