@@ -10,6 +10,8 @@
 // middle: behind it the next stage has landed, and everybody has the rest of this one in registers, so its slot is requested
 // again.  Where all rows are 16-byte aligned the copies go directly from memory to LDS; elsewhere they pass through registers, up to
 // four stages of loads ahead (1000 x 4096 x 4097 35.2 us, 1000 x 4096 x 4096 24).
+// Wavefronts that share out a stage's k instead of the tile's outputs (each byte of LDS is then read once, not twice) were slower: 64 x 64,
+// 250 x 4096 x 14336 25.4 -> 26.1 us, 512 x 4096 x 4096 15.7 -> 19.8 (one workgroup per compute unit for the longer stages).
 // No split of the reduction: its partial sums and second kernel cost 8 us and more, and where few tiles have a long reduction the
 // form for few rows, whose wavefronts share it out, is faster at any number of rows.
 #include "scaled_gemm_common.hpp"
