@@ -575,6 +575,68 @@ def test_block_in_a_graph_and_on_another_stream(calc, M):
         c.setStream(None)
 
 
+FORMS = [(4, 512, 512), (70, 4000, 512), (2001, 2001, 385), (4000, 4001, 512)]  # few rows, tiles of 64, 128 and 256
+
+
+def _products(seed):
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    cases = []
+    for M, N, K in FORMS:
+        x, w = (torch.randint(-127, 128, (r, K), generator=g, device="cuda", dtype=torch.int8) for r in (M, N))
+        out = torch.zeros(M, N, dtype=torch.int32, device="cuda")
+        cases.append((x, w, out, real_tensor(out, [N, M]), code_tensor(x, [K, M], "int8"), None, code_tensor(w, [K, N], "int8"), None))
+    torch.cuda.synchronize()
+    return cases
+
+
+def test_every_form_in_a_graph(calc):
+    import torch
+    cases = _products(1)
+    try:
+        side = torch.cuda.Stream()
+        calc.setStream(side.cuda_stream)
+        forms = set()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            for c in cases:
+                calc.scaledGemm(*c[3:])
+                forms.add(calc.lastContractionForm()["tile_rows"])
+        assert forms == {8, 64, 128, 256}
+        for k in range(3):
+            for x, _, out, *_ in cases:
+                x.add_(1)
+                out.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for x, w, out, *_ in cases:
+                assert torch.equal(out.double(), x.double() @ w.double().T), k
+    finally:
+        torch.cuda.synchronize()
+        calc.setStream(None)
+
+
+def test_two_calculators_at_once(calc):
+    """Calls of two handles on two streams, enqueued in turn, share nothing."""
+    import torch
+    from intel_gaudi3_software_amd import HipCalculator
+    second = HipCalculator()
+    try:
+        a, b = _products(2), _products(3)
+        for _ in range(5):
+            for p, q in zip(a, reversed(b)):
+                calc.scaledGemm(*p[3:])
+                second.scaledGemm(*q[3:])
+        calc.synchronize()
+        second.synchronize()
+        for x, w, out, *_ in a + b:
+            assert torch.equal(out.double(), x.double() @ w.double().T)
+    finally:
+        second.close()
+
+
 def test_own_stream_waits_for_torch(calc):
     """On its own stream the calculator waits for what torch's stream has enqueued."""
     import torch
