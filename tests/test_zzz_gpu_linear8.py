@@ -217,6 +217,26 @@ def test_norm_in_place_strided_and_gaps(calc):
     assert np.all(got[rest] == 85) and not _f64(scales)[R * Q:].any()
 
 
+@pytest.mark.parametrize("width", [100, 500, 4000, 5001, 14336, 20000, 70001])
+@pytest.mark.parametrize("place", ["x", "residual"])
+def test_norm_in_place_in_every_form(calc, width, place):
+    """The same bits as with an output of its own, ordinary rows and ones that are gone over twice."""
+    import torch
+    rng = np.random.default_rng(width)
+    x, r = (torch.from_numpy((rng.standard_normal((6, width)) * np.array([1, 1e30, 1e-30, 1, 0, 1])[:, None]).astype(np.float32)).cuda() for _ in range(2))
+    got = []
+    for own in (True, False):
+        X, R = x.clone(), r.clone()
+        out = torch.zeros_like(x) if own else X if place == "x" else R
+        codes, scales = torch.zeros(6, width, dtype=torch.uint8, device="cuda"), torch.zeros(6, device="cuda")
+        tx, tr = real_tensor(X, [width, 6]), real_tensor(R, [width, 6])
+        calc.rmsNormQuantize(code_tensor(codes, [width, 6], "e4m3"), scales, tx, None, tr, real_tensor(out, [width, 6]) if own else tx if place == "x" else tr)
+        calc.synchronize()
+        assert torch.equal(out, x + r)
+        got.append((codes, scales))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
 def test_broadcast_rows_and_no_rows(calc):
     import torch
     x = torch.randn(64, device="cuda")
