@@ -20,6 +20,8 @@ namespace
 constexpr int TM = 256, TN = 256, BK = 64, NST = 4, STAGE = (TM + TN) * BK;
 constexpr int LDS_BYTES = NST * STAGE; // 128 KiB
 #define FENCE __builtin_amdgcn_sched_barrier(0)
+// at most n of the wavefront's requests outstanding, and none of its LDS reads
+constexpr int landed_and_read(int n) { return vm_wait(n) & ~0x0F00; }
 
 __device__ __forceinline__ s_v8i read_frag(const char* st, int row0, int lane)
 {
@@ -87,8 +89,10 @@ __global__ __launch_bounds__(512, 2) void scaled_gemm_large_kernel(const ScaledG
     for (int j = 0; j < NJ; j++) fw[j] = read_frag(lds + TM * BK, wn * WC + j * 32, lane);
 
     // One stage: the products of stage t; behind the first, a wait until stage t + 1 has landed for every wavefront, then its
-    // fragments, each right after the last use of the register it goes to, and the requests of stage t + 4 into the slot of stage t,
-    // whose fragments every wavefront had read before that barrier
+    // fragments, each right after the last use of the register it goes to, and the requests of stage t + 4 into the slot of stage t.
+    // The wait is for this wavefront's reads of that slot as well: the last of them were issued at the end of the step before, and a
+    // barrier does not wait for them, while the requests behind it come from other wavefronts.  (The second product needs them anyway: no
+    // time is lost.  int8 4096^3 64.0 us, four products of fp8 2048 x 14336 x 4096 420.1, wait and barrier behind the second product 64.0 and 419.9.)
     auto step = [&](int t, auto waitc, auto loads, auto readnext) __attribute__((always_inline))
     {
         constexpr int  WAITC = decltype(waitc)::value;
@@ -132,7 +136,7 @@ __global__ __launch_bounds__(512, 2) void scaled_gemm_large_kernel(const ScaledG
         rw(1);
         FENCE;
     };
-    using WM = std::integral_constant<int, vm_wait((NST - 2) * NREQ)>;
+    using WM = std::integral_constant<int, landed_and_read((NST - 2) * NREQ)>;
     using T = std::true_type;
     using F = std::false_type;
     int t = 0;
@@ -146,10 +150,10 @@ __global__ __launch_bounds__(512, 2) void scaled_gemm_large_kernel(const ScaledG
         step(t, WM {}, T {}, T {});
         t++;
     }
-    step(t, std::integral_constant<int, vm_wait(2 * NREQ)> {}, F {}, T {});
-    step(t + 1, std::integral_constant<int, vm_wait(NREQ)> {}, F {}, T {});
-    step(t + 2, std::integral_constant<int, vm_wait(0)> {}, F {}, T {});
-    step(t + 3, std::integral_constant<int, vm_wait(0)> {}, F {}, F {});
+    step(t, std::integral_constant<int, landed_and_read(2 * NREQ)> {}, F {}, T {});
+    step(t + 1, std::integral_constant<int, landed_and_read(NREQ)> {}, F {}, T {});
+    step(t + 2, std::integral_constant<int, landed_and_read(0)> {}, F {}, T {});
+    step(t + 3, std::integral_constant<int, landed_and_read(0)> {}, F {}, F {});
     if (nk * BK < a.K)
     {
         // the codes behind the last whole stage, from registers
