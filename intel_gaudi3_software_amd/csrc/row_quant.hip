@@ -203,7 +203,8 @@ __device__ __forceinline__ void wave_reduce(float& sum, uint32_t& top)
 constexpr uint32_t INF_BITS = 0x7F800000u, LOW_BITS = 0x1F800000u /* 2^-64 */;
 
 // LANES per row: 16, 32 or 64, several rows per workgroup of 256; or 0, a workgroup per row.  Each lane holds NV times 8 elements of its
-// row in registers, at every (lanes per row x 8)-th place; NV 0: rows of any width, gone over again in memory for every pass.
+// row in registers, at every (lanes per row x 8)-th place; NV 0: rows of any width, gone over again in memory for every pass (places are
+// unsigned there: the step behind the last one of a row of nearly 2^31 elements leaves the signed range).
 template<int KIND, int TYPE, int LANES, int NV>
 __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void row_quant_kernel(const RowQuantArgs a)
 {
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void
         r /= a.n[1];
         return i0 * st[0] + i1 * st[1] + (r % a.n[2]) * st[2] + (r / a.n[2]) * st[3];
     };
-    auto load_gamma = [&](int e, float(&g)[VEC]) __attribute__((always_inline))
+    auto load_gamma = [&](uint32_t e, float(&g)[VEC]) __attribute__((always_inline))
     {
         if (!a.gamma)
         {
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void
         else
         {
 #pragma unroll 1
-            for (int e = lane * VEC; e < width; e += lanes * VEC)
+            for (uint32_t e = lane * VEC; e < (uint32_t) width; e += lanes * VEC)
             {
                 const auto xe = load8<TYPE>(a.x, x0 + e, width - e);
                 Raw<TYPE>  ye = xe;
@@ -365,9 +366,9 @@ __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void
     const float f = bad || top == 0u ? 0.0f : a.qmax / most;
     const float f_lo = bad || top == 0u ? 0.0f : __builtin_fmaf(-f, most, a.qmax) / most;
 
-    auto put = [&](int n, int e) __attribute__((always_inline))
+    auto put = [&](int n, uint32_t e) __attribute__((always_inline))
     {
-        const int left = width - e;
+        const int left = width - (int) e;
         if constexpr (KIND == ROWS_NORM_ADD)
             if (a.sum) store8<TYPE>(a.sum, r0 + e, left, rounded<TYPE>(s[n]));
         uint32_t c[2] = {0u, 0u};
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void
     else
     {
 #pragma unroll 1
-        for (int e = lane * VEC; e < width; e += lanes * VEC)
+        for (uint32_t e = lane * VEC; e < (uint32_t) width; e += lanes * VEC)
         {
             const auto xe = load8<TYPE>(a.x, x0 + e, width - e);
             Raw<TYPE>  ye = xe;
