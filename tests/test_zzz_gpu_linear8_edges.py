@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from intel_gaudi3_software_amd import abi
-from linear8_helpers import CODES, U, check_codes, code_tensor, code_values, real_tensor
+from linear8_helpers import U, check_codes, code_tensor, gate64, real_tensor
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,41 @@ def test_widest_rows(calc, width):
     # (at most 40 of a lane's squares are not zero: the roundings of the sum are those of a short row)
     top = np.max(np.abs(v)) / rms / 127
     assert abs(float(scales[0]) - top) <= 40 * U * top
+
+
+@pytest.mark.parametrize("gate,low,high,op", [("silu", -91.0, -87.01, abi.GATE_SILU), ("gelu", -10.15, -10.0, abi.GATE_GELU_TANH)])
+@pytest.mark.parametrize("width", [40, 700, 9000, 20001])
+def test_rows_in_the_gates_tail(calc, gate, low, high, op, width):
+    """Rows whose gates all lie where 1 + e^-g leaves the range of fp32 and g / (1 + e^-g) does not yet, beside ordinary and very large
+    values; one row has them among ordinary gates, with factors that make up for them."""
+    import torch
+    rng = np.random.default_rng(width)
+    g = rng.uniform(low, high, (4, width)).astype(np.float32)
+    x = (rng.standard_normal((4, width)) * np.array([1.0, 1e10, 1e37, 1.0])[:, None]).astype(np.float32)
+    plain = rng.random(width) < 0.5
+    g[3, plain] = rng.standard_normal(int(plain.sum()))
+    x[3, ~plain] *= np.float32(3e36)
+    codes, scales = torch.zeros(4, width, dtype=torch.uint8, device="cuda"), torch.zeros(4, device="cuda")
+    calc.quantizeRows(code_tensor(codes, [width, 4], "e5m2"), scales, real_tensor(torch.from_numpy(x).cuda(), [width, 4]), real_tensor(torch.from_numpy(g).cuda(), [width, 4]), op)
+    calc.synchronize()
+    # fp32 roundings: those of the gate elsewhere (12; the gelu's argument has five, which its size, at most 91 here, magnifies), and the
+    # factor's argument, its exponential and its product (4)
+    roundings = 16 if gate == "silu" else 16 + 5 * 91
+    v = gate64(g.astype(np.float64), gate) * x.astype(np.float64)
+    check_codes(v, _codes_of(codes), scales.cpu().double().numpy(), "e5m2", roundings, roundings + 2)
+
+
+def test_gates_where_fp32_ends(calc):
+    """Gated values below 2^-126 have a denormal's bits, those below 2^-150 are zero, whatever multiplies them."""
+    import torch
+    g = np.array([-95.0, -100.0, -103.0, -110.0, -200.0, -1e30], np.float32)
+    scales, codes = torch.zeros(6, device="cuda"), torch.zeros(6, 8, dtype=torch.uint8, device="cuda")
+    gt, x = torch.from_numpy(np.repeat(g[:, None], 8, 1)).cuda(), torch.full((6, 8), 1e30, device="cuda")
+    calc.quantizeRows(code_tensor(codes, [8, 6], "int8"), scales, real_tensor(x, [8, 6]), real_tensor(gt, [8, 6]), abi.GATE_SILU)
+    calc.synchronize()
+    with np.errstate(over="ignore"):
+        want = np.abs(gate64(g.astype(np.float64), "silu"))
+    got = scales.cpu().double().numpy() * 127 / np.float64(np.float32(1e30))
+    assert np.all(np.abs(got - want) <= 16 * U * want + 2.0 ** -149), (got, want)
+    assert np.all(got[3:] == 0) and np.all(got[:3] > 0)
+    assert np.all(_codes_of(codes).view(np.int8)[:3] == -127) and not codes[3:].any()
