@@ -557,9 +557,9 @@ int mme_hip_quantize_rows_dev(mme_hip_handle        h,
  *     s = x + residual (fp32),   residual_out = s rounded to x's type,   v_i = s_i gamma_i / sqrt(mean(s^2) + eps)
  * The norm works on s before it is rounded.  residual and residual_out (types and sizes of x) may be NULL: s = x, and the sum is
  * not kept; residual_out needs a residual and may be x or residual themselves (the same descriptor: in place).  gamma: sizes[0]
- * elements in one row, of x's type or fp32, NULL for ones.  eps: finite, >= 0.  A row whose s or s gamma holds an inf or NaN
- * has the scale NaN and codes 0 (residual_out is written as it is); finite values of any size are normalised without
- * overflow.  A row of zeros has the scale 0, also with eps 0.
+ * elements in one row, of x's type or fp32, NULL for ones.  eps: finite, >= 0.  A row whose s holds an inf or NaN, or whose gamma does,
+ * has the scale NaN and codes 0 (residual_out is written as it is); finite values and gammas of any size are normalised without
+ * overflow, and without underflow as long as the scale is not below 2^-126.  A row of zeros has the scale 0, also with eps 0.
  */
 int mme_hip_rms_norm_quantize_dev(mme_hip_handle        h,
                                   const mme_hip_tensor* out,

@@ -11,9 +11,10 @@
 //
 // Arithmetic is fp32 (the scale, one number per row, is finished in fp64).  Rounded to fewer bits: the codes, and the
 // residual sum in its own type; the norm works on the sum before that rounding.
-// Rows whose values leave the comfortable middle of the fp32 range (squares or products that overflow, a maximum below 2^-64
-// whose reciprocal would) are gone over once more with the values multiplied by 2^-96 or 2^96, exactly.  A row that holds an
-// inf or NaN gets the scale NaN and codes 0; a row of zeros the scale 0 and codes 0.
+// Rows whose values leave the comfortable middle of the fp32 range (squares or products with gamma that overflow, a maximum below 2^-64
+// whose reciprocal would) are gone over once more, with the squared values multiplied by 2^-96 or 2^96 and the products by 2^-132 or 2^144,
+// exactly.  A row that holds an inf or NaN (a gated product that overflows is one) gets the scale NaN and codes 0; a row of zeros the scale
+// 0 and codes 0.
 #include "mme_numeric.hpp"
 #include "scaled_kernels.hpp"
 
@@ -277,34 +278,36 @@ __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void
             for (int i = 0; i < VEC; i++) s[i] = KIND == ROWS_NORM_ADD ? value<TYPE>(x, i) + value<TYPE>(y, i) : value<TYPE>(x, i);
         }
     };
-    // u: what the codes stand for up to a factor of the row; fu: a power of two it is multiplied by (1 but for rows gone over again)
-    auto make_u = [&](const float(&s)[VEC], const float(&g)[VEC], float fu, float(&u)[VEC]) __attribute__((always_inline))
+    // u: what the codes stand for up to a factor of the row; hu: a power of two that it is multiplied by twice (1 but for rows gone over again)
+    auto make_u = [&](const float(&s)[VEC], const float(&g)[VEC], float hu, float(&u)[VEC]) __attribute__((always_inline))
     {
-        if (fu == 1.0f)
+        if (hu == 1.0f)
         {
 #pragma unroll
             for (int i = 0; i < VEC; i++) u[i] = NORM ? s[i] * g[i] : s[i];
         }
         else if (NORM)
         {
-            // the power goes to the factor that it takes towards one: nothing overflows or vanishes on the way
+            // the powers go to the smaller factor where they enlarge, to the larger one where they diminish: with 2^144 (all products
+            // below 2^-64, so the smaller factor below 2^-32) and 2^-132 (the largest product at least 2^128) nothing overflows on the
+            // way, and what vanishes is nothing beside the largest
 #pragma unroll
             for (int i = 0; i < VEC; i++)
             {
-                const bool small = __builtin_fabsf(s[i]) < 1.0f, to_s = small == (fu > 1.0f);
-                u[i] = (to_s ? s[i] * fu : s[i]) * (to_s ? g[i] : g[i] * fu);
+                const bool to_s = (__builtin_fabsf(s[i]) < __builtin_fabsf(g[i])) == (hu > 1.0f);
+                u[i] = (to_s ? s[i] : g[i]) * hu * hu * (to_s ? g[i] : s[i]);
             }
         }
         else
         {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) u[i] = s[i] * fu;
+            for (int i = 0; i < VEC; i++) u[i] = s[i] * hu * hu;
         }
     };
-    auto gather = [&](const float(&s)[VEC], const float(&g)[VEC], float fs, float fu, float& sum, uint32_t& top) __attribute__((always_inline))
+    auto gather = [&](const float(&s)[VEC], const float(&g)[VEC], float fs, float hu, float& sum, uint32_t& top) __attribute__((always_inline))
     {
         float u[VEC];
-        make_u(s, g, fu, u);
+        make_u(s, g, hu, u);
         if constexpr (NORM)
         {
 #pragma unroll
@@ -350,14 +353,14 @@ __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void
 #pragma unroll
         for (int n = 0; n < NV; n++) make_s(x[n], y[n], s[n]);
     }
-    auto pass = [&](float fs, float fu, float& sum, uint32_t& top) __attribute__((always_inline))
+    auto pass = [&](float fs, float hu, float& sum, uint32_t& top) __attribute__((always_inline))
     {
         sum = 0.0f;
         top = 0u;
         if constexpr (NV > 0)
         {
 #pragma unroll
-            for (int n = 0; n < NV; n++) gather(s[n], gamma[n], fs, fu, sum, top);
+            for (int n = 0; n < NV; n++) gather(s[n], gamma[n], fs, hu, sum, top);
         }
         else
         {
@@ -369,21 +372,21 @@ __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void
                 if constexpr (TWO) ye = load8<TYPE>(a.second, y0 + e, width - e);
                 make_s(xe, ye, s[0]);
                 if constexpr (NORM) load_gamma(e, gamma[0]);
-                gather(s[0], gamma[0], fs, fu, sum, top);
+                gather(s[0], gamma[0], fs, hu, sum, top);
             }
         }
         reduce(sum, top);
     };
-    float    fs = 1.0f, fu = 1.0f, sum;
+    float    fs = 1.0f, hu = 1.0f, sum;
     uint32_t top;
     pass(1.0f, 1.0f, sum, top);
     const bool odd = top >= INF_BITS || top < LOW_BITS || (NORM && !(sum < 0x1p+126f && sum > 0x1p-100f)); // (the same in every lane of the row)
     if (LANES ? __any(odd && live) : odd)
     {
         // (a wavefront with several rows goes over all of them, those that need it not with factors of one)
-        fu = top >= INF_BITS ? 0x1p-96f : (top < LOW_BITS ? 0x1p+96f : 1.0f);
+        hu = top >= INF_BITS ? 0x1p-66f : (top < LOW_BITS ? 0x1p+72f : 1.0f);
         if (NORM) fs = !(sum < 0x1p+126f) ? 0x1p-96f : (sum > 0x1p-100f ? 1.0f : 0x1p+96f);
-        pass(fs, fu, sum, top);
+        pass(fs, hu, sum, top);
     }
     const bool  bad = top >= INF_BITS || (NORM && !(sum < __uint_as_float(INF_BITS)));
     const float most = __uint_as_float(top);
@@ -400,7 +403,7 @@ __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void
         if (!bad)
         {
             float u[VEC];
-            make_u(s[n], gamma[n], fu, u);
+            make_u(s[n], gamma[n], hu, u);
             if (a.code == CODE_INT8)
             {
                 // added to 1.5 x 2^23 the product is rounded once, to a whole number (127 for the largest: f is off by less than
@@ -474,7 +477,7 @@ __global__ __launch_bounds__(LANES ? 256 : NV == 1 || NV == 4 ? 512 : 1024) void
     }
     if (lane == 0 && live)
     {
-        double sc = (double) most / (double) a.qmax * a.fold / (double) fu;
+        double sc = (double) most / (double) a.qmax * a.fold / ((double) hu * (double) hu);
         if (NORM)
         {
             const double ms = (double) sum / ((double) fs * (double) fs) / (double) width;

@@ -80,3 +80,23 @@ def test_gates_where_fp32_ends(calc):
     assert np.all(np.abs(got - want) <= 16 * U * want + 2.0 ** -149), (got, want)
     assert np.all(got[3:] == 0) and np.all(got[:3] > 0)
     assert np.all(_codes_of(codes).view(np.int8)[:3] == -127) and not codes[3:].any()
+
+
+@pytest.mark.parametrize("width", [40, 700, 5000, 9000, 20001])
+@pytest.mark.parametrize("factor,gamma", [(1e37, 1e37), (1e37, 1e20), (1e-36, 1e-36), (1e-20, 1e-36), (1e-37, 1e37), (1e37, 1e-37)])
+def test_norm_of_values_and_gammas_of_any_size(calc, width, factor, gamma):
+    """Products of a value and its gamma may lie anywhere, as long as the normalised value is one of fp32's."""
+    import torch
+    rng = np.random.default_rng(width)
+    x = (rng.standard_normal((3, width)) * factor).astype(np.float32)
+    g = (rng.uniform(0.5, 2.0, width) * gamma).astype(np.float32)
+    g[::7] *= np.float32(1e-3)
+    codes, scales = torch.zeros(3, width, dtype=torch.uint8, device="cuda"), torch.zeros(3, device="cuda")
+    X, G = real_tensor(torch.from_numpy(x).cuda(), [width, 3]), real_tensor(torch.from_numpy(g).cuda(), [width])
+    for kind in ("int8", "e4m3"):
+        calc.rmsNormQuantize(code_tensor(codes, [width, 3], kind), scales, X, G, eps=0.0)
+        calc.synchronize()
+        s = x.astype(np.float64)
+        v = s * g.astype(np.float64)[None] / np.sqrt(np.mean(s * s, axis=1, keepdims=True))
+        # (roundings: the product, its power of two exactly, the quotient in two parts, the last one; the sum's as in the other tests, halved by the root)
+        check_codes(v, _codes_of(codes), scales.cpu().double().numpy(), kind, 4, 8 + ((16 if width <= 16384 else 24) + 16) / 2)
