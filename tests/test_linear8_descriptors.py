@@ -1,0 +1,38 @@
+"""Python descriptors of the 8-bit linear layer (no GPU): what the calls are told about a tensor stays inside its buffer."""
+import numpy as np
+import pytest
+
+from intel_gaudi3_software_amd import HipCalculator, MMEStackException, MmeSimTensor, abi
+
+
+def told(t):
+    """The strides that the 8-bit linear layer's entry points are given."""
+    return list(t._ref._obj.strides)
+
+
+def last(t, strides):
+    return sum(st * (sz - 1) for st, sz in zip(strides, t.sizes))
+
+
+def test_a_stride_of_zero_repeats_the_row():
+    row = np.zeros(64, np.float32)
+    t = MmeSimTensor([64, 9], 2, abi.FP32, row, strides=[1, 0])
+    assert told(t)[:2] == [1, 0] and last(t, told(t)) == 63 and t._ref._obj.data == row.ctypes.data
+    planes = np.zeros(64 * 3, np.float32)
+    t = MmeSimTensor([64, 3, 5], 3, abi.FP32, planes, strides=[1, 64, 0])
+    assert told(t)[:3] == [1, 64, 0] and last(t, told(t)) == 191
+    t = MmeSimTensor([64, 5, 3], 3, abi.FP32, planes, strides=[1, 0, 64])
+    assert told(t)[:3] == [1, 0, 64]
+    # the other entry points take such strides for dense ones: not in a buffer that has no room for that
+    t = MmeSimTensor([64, 9], 2, abi.FP32, row, strides=[1, 0])
+    calc = HipCalculator.__new__(HipCalculator)
+    with pytest.raises(MMEStackException) as e:
+        calc._placement(t)
+    assert e.value.status == abi.EINVAL
+    t = MmeSimTensor([64, 9], 2, abi.FP32, np.zeros(64 * 9, np.float32), strides=[1, 0])
+    assert calc._placement(t) is False and list(t.desc.strides)[:2] == [1, 64] and told(t)[:2] == [1, 0]
+    # (a dimension of one index or none has no stride to speak of)
+    t = MmeSimTensor([64, 9, 1], 3, abi.FP32, np.zeros(64 * 9, np.float32), strides=[1, 64, 0, 0, 0])
+    assert told(t) == list(t.desc.strides) == [1, 64, 576, 576, 576]
+    t = MmeSimTensor([64, 0], 2, abi.FP32)
+    assert told(t) == list(t.desc.strides)

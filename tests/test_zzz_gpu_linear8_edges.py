@@ -100,3 +100,24 @@ def test_norm_of_values_and_gammas_of_any_size(calc, width, factor, gamma):
         v = s * g.astype(np.float64)[None] / np.sqrt(np.mean(s * s, axis=1, keepdims=True))
         # (roundings: the product, its power of two exactly, the quotient in two parts, the last one; the sum's as in the other tests, halved by the root)
         check_codes(v, _codes_of(codes), scales.cpu().double().numpy(), kind, 4, 8 + ((16 if width <= 16384 else 24) + 16) / 2)
+
+
+def test_rows_repeated_by_a_stride_of_zero(calc):
+    """A tensor of one row in memory and many by its strides, as an operand of each call."""
+    import torch
+    x = torch.randn(64, device="cuda")
+    codes, one = torch.zeros(9, 64, dtype=torch.uint8, device="cuda"), torch.zeros(1, 64, dtype=torch.uint8, device="cuda")
+    scales, single = torch.zeros(9, device="cuda"), torch.zeros(1, device="cuda")
+    many = real_tensor(x, [64, 9], strides=[1, 0])
+    calc.quantizeRows(code_tensor(one, [64, 1], "int8"), single, real_tensor(x, [64, 1]))
+    calc.quantizeRows(code_tensor(codes, [64, 9], "int8"), scales, many)
+    calc.synchronize()
+    assert torch.equal(codes, one.expand(9, 64)) and torch.equal(scales, single.expand(9))
+    calc.rmsNormQuantize(code_tensor(codes, [64, 9], "int8"), scales, many)
+    calc.synchronize()
+    assert torch.equal(codes, one.expand(9, 64)) and torch.all(scales == scales[0])
+    out = torch.zeros(9, 9, dtype=torch.int32, device="cuda")
+    calc.scaledGemm(real_tensor(out, [9, 9]), code_tensor(one, [64, 9], "int8", strides=[1, 0]), None, code_tensor(codes, [64, 9], "int8"), None)
+    calc.synchronize()
+    v = one.view(torch.int8).long()
+    assert torch.all(out == (v * v).sum())
