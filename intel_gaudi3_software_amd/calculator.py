@@ -57,6 +57,8 @@ class MmeSimTensor:
                 strides.append(strides[-1] * self.sizes[len(strides) - 1])
         self.strides = strides
         span = max(st * sz for st, sz in zip(self.strides, self.sizes))
+        if min(self.sizes) > 0:  # (rows of two dimensions that lie between or on each other reach further than either)
+            span = max(span, 1 + sum(st * (sz - 1) for st, sz in zip(self.strides, self.sizes)))
         self.is_device = False
         if data is None:
             data = np.zeros(max(span, 1), dtype=abi.DTYPE_NUMPY[dtype])

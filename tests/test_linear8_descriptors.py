@@ -36,3 +36,15 @@ def test_a_stride_of_zero_repeats_the_row():
     assert told(t) == list(t.desc.strides) == [1, 64, 576, 576, 576]
     t = MmeSimTensor([64, 0], 2, abi.FP32)
     assert told(t) == list(t.desc.strides)
+
+
+def test_overlapping_rows_stay_inside_the_buffer():
+    """Input rows may share memory: the buffer has to hold the last element of the last row, which no single dimension shows."""
+    for sizes, strides in (([64, 9, 9], [1, 8, 8]), ([16, 4, 4], [1, 16, 24]), ([8, 3, 1, 5], [1, 5, 15, 7])):
+        need = 1 + sum(st * (sz - 1) for st, sz in zip(strides, sizes))
+        assert need > max(st * sz for st, sz in zip(strides, sizes))
+        t = MmeSimTensor(sizes, len(sizes), abi.FP32, np.zeros(need, np.float32), strides=strides)
+        assert last(t, told(t)) == need - 1
+        with pytest.raises(ValueError):
+            MmeSimTensor(sizes, len(sizes), abi.FP32, np.zeros(need - 1, np.float32), strides=strides)
+        assert MmeSimTensor(sizes, len(sizes), abi.FP32, strides=strides).data().size >= need
