@@ -277,7 +277,7 @@ class HipCalculator:
     def setStream(self, hip_stream):
         """Enqueue on a caller-owned stream (0 / None: back to the calculator's own).  With a caller-owned stream the
         ordering against the producers of the operands is the caller's business; on its own stream the calculator waits,
-        on the device, for what torch's current stream has enqueued so far before every call on torch tensors."""
+        on the device, for what torch's current stream of that device has enqueued so far before every call on torch tensors."""
         self._check(self._lib.mme_hip_set_stream(self._h, hip_stream))
         self._caller_stream = bool(hip_stream)
 
@@ -290,8 +290,8 @@ class HipCalculator:
             return
         import torch
         ev = torch.cuda.Event()
-        ev.record()
-        torch.cuda.ExternalStream(self.stream()).wait_event(ev)
+        ev.record(torch.cuda.current_stream(self._gpu))  # (of the operands' device, whichever is current)
+        torch.cuda.ExternalStream(self.stream(), device=self._gpu).wait_event(ev)
         self._in_flight.extend(t for t in device_tensors if t is not None and getattr(t, "is_cuda", False))
         if len(self._in_flight) > 512:
             self.synchronize()

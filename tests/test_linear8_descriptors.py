@@ -48,3 +48,29 @@ def test_overlapping_rows_stay_inside_the_buffer():
         with pytest.raises(ValueError):
             MmeSimTensor(sizes, len(sizes), abi.FP32, np.zeros(need - 1, np.float32), strides=strides)
         assert MmeSimTensor(sizes, len(sizes), abi.FP32, strides=strides).data().size >= need
+
+
+def test_own_stream_waits_for_the_stream_of_its_own_device(monkeypatch):
+    """The operands are written on the current stream of their device, which need not be the current device's."""
+    torch = pytest.importorskip("torch")
+    seen = []
+
+    class Event:
+        def record(self, stream=None):
+            seen.append(("record", stream))
+
+    class External:
+        def __init__(self, pointer, device=None):
+            seen.append(("stream", pointer, device))
+
+        def wait_event(self, event):
+            seen.append(("wait", type(event)))
+
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", External)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: "stream of device %s" % device)
+    calc = HipCalculator.__new__(HipCalculator)
+    calc._caller_stream, calc._in_flight, calc._gpu = False, [], 3
+    monkeypatch.setattr(HipCalculator, "stream", lambda self: 77)
+    calc._after_torch()
+    assert seen == [("record", "stream of device 3"), ("stream", 77, 3), ("wait", Event)]
