@@ -25,13 +25,12 @@ def build(with_ref=True):
     """Compile the checkers (gcc / g++ through oracle/Makefile).  The reference library is built only where the
     reference tree is present."""
     subprocess.check_call(["make", "-s", "-C", _HERE, "oracle"])
-    if with_ref and os.path.isdir(os.environ.get("MME_REFERENCE_ROOT", "/root/reference")):
-        subprocess.check_call(["make", "-s", "-j8", "-C", _HERE, "ref",
-                               "REF=" + os.environ.get("MME_REFERENCE_ROOT", "/root/reference")])
+    root = os.environ.get("MME_REFERENCE_ROOT", "/root/reference")
+    if with_ref and os.path.isfile(os.path.join(root, "mme", "mme_reference", "mme_reference_impl.cpp")):
+        subprocess.check_call(["make", "-s", "-j8", "-C", _HERE, "ref", "REF=" + root])
         # the drop-in demonstration links the MI355X library: built only where that has been built
         if os.path.exists(os.path.join(_HERE, "..", "intel_gaudi3_software_amd", "csrc", "libmme_hip.so")):
-            subprocess.check_call(["make", "-s", "-j8", "-C", _HERE, "ref_dropin",
-                                   "REF=" + os.environ.get("MME_REFERENCE_ROOT", "/root/reference")])
+            subprocess.check_call(["make", "-s", "-j8", "-C", _HERE, "ref_dropin", "REF=" + root])
 
 
 def oracle():
