@@ -133,6 +133,8 @@ __device__ __forceinline__ void read_b_kc(FR& f, int j, const char* st, int cb0,
 // s_waitcnt immediate that waits until at most n of this wavefront's memory requests are outstanding and leaves the other
 // counters alone (gfx9 encoding: vmcnt[3:0] | expcnt[6:4] | lgkmcnt[11:8] | vmcnt[5:4] << 14)
 constexpr int vm_wait(int n) { return 0x0F70 | (n & 15) | ((n >> 4) << 14); }
+// the same, and none of its LDS accesses
+constexpr int landed_and_read(int n) { return vm_wait(n) & ~0x0F00; }
 
 // The problem description is read in place from the kernarg segment, field by field where the code needs it: every 64-byte
 // line touched for the first time (tile set-up, gather set-up, epilogue) would be a miss of its own, one memory latency
@@ -731,7 +733,10 @@ __device__ __forceinline__ void gemm_fast_body_impl(KARG GemmProblem& g)
     // One stage: 8 MFMAs; after the first one wait until stage t+1 has landed in every wavefront's view (WAITC leaves the
     // younger stages in flight); each fragment register is refilled from stage t+1 right after its last use in stage t (the
     // other wavefront on the SIMD covers the tail of that latency); request stage t+4 into the slot of stage t, whose
-    // fragments every wavefront read during the previous step (the barrier above orders those reads before this request).
+    // fragments every wavefront read during the previous step: the barrier orders those reads before this request, because the wait in
+    // front of it is for them too (a barrier waits for no LDS access, and the last fragments were asked for at the very end of
+    // that step).  The next products need them in any case: fp8 4096^3 58.9 us, 3x3 dedx and dedw of 32 images of 28 x 28 x 256 784 and
+    // 658 TFLOP/s; with wait and barrier behind the second product instead 58.8 us, 781 and 637.
     int  slot_of_step = 0; // t mod NST of the next step
     auto step = [&](int t, auto waitc, auto loads, auto readnext) __attribute__((always_inline))
     {
@@ -817,7 +822,7 @@ __device__ __forceinline__ void gemm_fast_body_impl(KARG GemmProblem& g)
     };
     // at the wait of step t the stages t+1 .. t+NST-1 have been requested; stage t+1 is needed, so the younger NST-2 stages of
     // this wavefront's requests may stay in flight
-    using WM = std::integral_constant<int, vm_wait((NST - 2) * NREQ)>;
+    using WM = std::integral_constant<int, landed_and_read((NST - 2) * NREQ)>;
     using T = std::true_type;
     using F = std::false_type;
     int t = 0;
@@ -847,14 +852,14 @@ __device__ __forceinline__ void gemm_fast_body_impl(KARG GemmProblem& g)
     auto drain = [&](auto ic) __attribute__((always_inline))
     {
         constexpr int I = decltype(ic)::value;
-        if constexpr (I < NST - 1) step(t + I, std::integral_constant<int, vm_wait((NST - 2 - I) * NREQ)> {}, F {}, T {});
+        if constexpr (I < NST - 1) step(t + I, std::integral_constant<int, landed_and_read((NST - 2 - I) * NREQ)> {}, F {}, T {});
     };
     if constexpr (NST == 4)
     {
-        step(t, std::integral_constant<int, vm_wait(2 * NREQ)> {}, F {}, T {});
-        step(t + 1, std::integral_constant<int, vm_wait(NREQ)> {}, F {}, T {});
-        step(t + 2, std::integral_constant<int, vm_wait(0)> {}, F {}, T {});
-        step(t + 3, std::integral_constant<int, vm_wait(0)> {}, F {}, F {});
+        step(t, std::integral_constant<int, landed_and_read(2 * NREQ)> {}, F {}, T {});
+        step(t + 1, std::integral_constant<int, landed_and_read(NREQ)> {}, F {}, T {});
+        step(t + 2, std::integral_constant<int, landed_and_read(0)> {}, F {}, T {});
+        step(t + 3, std::integral_constant<int, landed_and_read(0)> {}, F {}, F {});
     }
     else
     {
@@ -863,7 +868,7 @@ __device__ __forceinline__ void gemm_fast_body_impl(KARG GemmProblem& g)
         drain(std::integral_constant<int, 2> {});
         drain(std::integral_constant<int, 3> {});
         drain(std::integral_constant<int, 4> {});
-        step(t + NST - 1, std::integral_constant<int, vm_wait(0)> {}, F {}, F {});
+        step(t + NST - 1, std::integral_constant<int, landed_and_read(0)> {}, F {}, F {});
     }
 #undef MMA
 #undef RA

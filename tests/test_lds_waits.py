@@ -38,24 +38,31 @@ def code_objects(path):
 HEAD = re.compile(r"^([0-9a-f]+) <(.*)>:$")
 LINE = re.compile(r"^\t(\S+)(.*?)// ([0-9A-F]+):.*?(?:<.*\+0x([0-9a-f]+)>)?$")
 LGKM = re.compile(r"lgkmcnt\((\d+)\)")
-ENDS = ("s_branch", "s_endpgm", "s_setpc_b64")
+ENDS = ("s_branch", "s_endpgm", "s_setpc_b64", "always")
+ZERO = re.compile(r"^\ts_mov_b64 (s\[\d+:\d+\]), 0 +// ([0-9A-F]+):")
 
 
 def functions(text):
-    """(name, [(address, mnemonic, operands, branch target)]) of every function, only what the analysis looks at."""
-    name, start, lines = None, 0, []
+    """(name, [(address, mnemonic, operands, branch target)]) of every function, only what the analysis looks at.  A condition that is set
+    to zero right in front of the branch on it (how the compiler ends the first of two alternatives, the second of which others
+    enter at the branch) is a branch that is always taken by whoever comes past the setting: "always"."""
+    name, start, lines, before = None, 0, [], ("", "")
     for line in text.splitlines():
         if not line.startswith("\t"):
             m = HEAD.match(line)
             if m:
                 if name:
                     yield name, lines
-                name, start, lines = m.group(2), int(m.group(1), 16), []
+                name, start, lines, before = m.group(2), int(m.group(1), 16), [], ("", "")
             continue
         if line.startswith(("\tds_", "\ts_waitcnt", "\ts_barrier", "\ts_cbranch", "\ts_branch", "\ts_endpgm", "\ts_setpc", "\tglobal_load_lds", "\tbuffer_load")):
             m = LINE.match(line)
             target = start + int(m.group(4), 16) if m.group(4) else start if "branch" in m.group(1) and "// " in line and line.endswith(">") else None
+            zero = ZERO.match(before[0])
+            if m.group(1) == "s_cbranch_vccz" and zero and before[1].startswith("\ts_and_b64 vcc, exec, %s " % zero.group(1)):
+                lines.append((int(zero.group(2), 16), "always", "", target))
             lines.append((int(m.group(3), 16), m.group(1), m.group(2), target))
+        before = (before[1], line)
     if name:
         yield name, lines
 
@@ -135,9 +142,27 @@ def test_the_analysis_itself():
     fixed = listing.replace("s_waitcnt vmcnt(8) ", "s_waitcnt vmcnt(8) lgkmcnt(0) ").replace("\ts_cbranch_scc1", "\ts_waitcnt lgkmcnt(0) // 00000000101C:\n\ts_cbranch_scc1")
     (_, lines), = functions(fixed)
     assert list(outstanding_at_barriers(lines).values()) == [0, 0]
+    # two alternatives: the end of the first never enters the second, which is entered at the branch
+    listing = ("0000000000002000 <k>:\n"
+               "\ts_cbranch_scc0 9                                           // 000000002000: BF840009 <k+0x18>\n"
+               "\tds_write_b128 v4, v[0:3]                                   // 000000002004: D9BE0000\n"
+               "\ts_mov_b64 s[6:7], 0                                        // 000000002010: BE860180\n"
+               "\ts_and_b64 vcc, exec, s[6:7]                                // 000000002018: 86EA067E\n"
+               "\ts_cbranch_vccz 3                                           // 00000000201C: BF860003 <k+0x28>\n"
+               "\ts_barrier                                                  // 000000002020: BF8A0000\n"
+               "\ts_endpgm                                                   // 000000002028: BF810000\n")
+    (_, lines), = functions(listing)
+    assert list(outstanding_at_barriers(lines).values()) == [0]
+    (_, lines), = functions(listing.replace("s_mov_b64 s[6:7], 0 ", "s_mov_b64 s[6:7], -1"))
+    assert list(outstanding_at_barriers(lines).values()) == [1]
 
 
 def test_scaled_product_has_no_lds_access_in_flight_at_a_barrier(kernels):
     mine = {n: k for n, k in kernels.items() if "scaled_gemm" in n}
     assert len(mine) > 60 and any("large" in n for n in mine) and all(k[1] for n, k in mine.items() if "large" in n)
     assert not {n: k[0] for n, k in mine.items() if max(k[0])}
+
+
+def test_no_kernel_has_an_lds_access_in_flight_at_a_barrier(kernels):
+    assert sum(k[1] for k in kernels.values()) > 150  # (kernels that request copies to LDS)
+    assert not {n: k[0] for n, k in kernels.items() if max(k[0])}
