@@ -186,34 +186,35 @@ __device__ __forceinline__ void store_scaled4(const ScaledGemmArgs& a, const Bat
 {
     const long long e = o.out + (long long) m * a.out_ld + n;
     const bool      whole = n + 4 <= a.N;
-    uint32_t        word[4];
+    float           v[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        word[i] = a.out_type == SCALED_OUT_INT32 ? (uint32_t) (int) sum[i] : __float_as_uint(scaled_value(sum[i], a.alpha, sx, c.sw.v[i], c.bias.v[i], a.bias != nullptr));
-    if (a.out_type == SCALED_OUT_FP32 || a.out_type == SCALED_OUT_INT32)
-    {
-        uint32_t* p = (uint32_t*) a.out + e;
-        if (whole) *(u128_any*) p = u128_any {{word[0], word[1], word[2], word[3]}};
-        else
+    for (int i = 0; i < 4; i++) v[i] = scaled_value(sum[i], a.alpha, sx, c.sw.v[i], c.bias.v[i], a.bias != nullptr);
+    if constexpr (std::is_same<S, int>::value) // (fp8 operands have 16-bit outputs)
+        if (a.out_type == SCALED_OUT_FP32 || a.out_type == SCALED_OUT_INT32)
         {
+            uint32_t* p = (uint32_t*) a.out + e;
+            uint32_t  word[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (n + i < a.N) p[i] = word[i];
+            for (int i = 0; i < 4; i++) word[i] = a.out_type == SCALED_OUT_INT32 ? (uint32_t) sum[i] : __float_as_uint(v[i]);
+            if (whole) *(u128_any*) p = u128_any {{word[0], word[1], word[2], word[3]}};
+            else
+            {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (n + i < a.N) p[i] = word[i];
+            }
+            return;
         }
-    }
+    uint16_t* p = (uint16_t*) a.out + e;
+    uint32_t  half[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) half[i] = to_half(v[i], a.out_type);
+    if (whole) *(u64_any*) p = u64_any {{half[0] | (half[1] << 16), half[2] | (half[3] << 16)}};
     else
     {
-        uint16_t* p = (uint16_t*) a.out + e;
-        uint32_t  half[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) half[i] = to_half(__uint_as_float(word[i]), a.out_type);
-        if (whole) *(u64_any*) p = u64_any {{half[0] | (half[1] << 16), half[2] | (half[3] << 16)}};
-        else
-        {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (n + i < a.N) p[i] = (uint16_t) half[i];
-        }
+        for (int i = 0; i < 4; i++)
+            if (n + i < a.N) p[i] = (uint16_t) half[i];
     }
 }
 __device__ __forceinline__ float scale_of_row(const ScaledGemmArgs& a, const BatchOffsets& o, int m) { return a.sx ? a.sx[o.sx + min(m, a.M - 1)] : 1.0f; }
