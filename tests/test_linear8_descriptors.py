@@ -74,3 +74,17 @@ def test_own_stream_waits_for_the_stream_of_its_own_device(monkeypatch):
     monkeypatch.setattr(HipCalculator, "stream", lambda self: 77)
     calc._after_torch()
     assert seen == [("record", "stream of device 3"), ("stream", 77, 3), ("wait", Event)]
+
+
+def test_windows_of_windows():
+    """A window's address and strides, windows inside it, and those that leave the buffer."""
+    t = MmeSimTensor([20, 3], 2, abi.FP32)
+    w = t.window(10, [10, 3])
+    assert w.desc.data == t.desc.data + 40 and list(w.desc.strides)[:2] == [1, 20] and w.getSizes()[:2] == [10, 3]
+    assert w.window(3, [7, 3]).desc.data == t.desc.data + 52
+    assert list(t.window(0, [20, 9], [1, 0, 0, 0, 0]).desc.strides) == [1, 0, 0, 0, 0]
+    for bad in ((11, [10, 3]), (0, [20, 4]), (-1, [10, 3])):
+        with pytest.raises(ValueError):
+            t.window(*bad)
+    with pytest.raises(ValueError):
+        w.window(3, [8, 3])
