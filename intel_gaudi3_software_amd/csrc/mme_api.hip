@@ -239,11 +239,20 @@ uint64_t span_elements(const mme_hip_tensor* t)
     for (int d = 0; d < 5; d++) m = std::max<uint64_t>(m, (uint64_t) t->strides[d] * t->sizes[d]);
     return m;
 }
-// dims 1..4 enumerate rows of one dense-pitched matrix: stride[d+1] == stride[d] * size[d]
+// dims 1..4 enumerate rows of one dense-pitched matrix: stride[d+1] == stride[d] * size[d], over the dimensions of one index too (whose own
+// stride says nothing, so a dimension behind them has to follow from the last one that has several as well)
 bool rows_collapsible(const mme_hip_tensor* t)
 {
-    for (int d = 1; d < 4; d++)
-        if (t->sizes[d + 1] > 1 && (uint64_t) t->strides[d + 1] != (uint64_t) t->strides[d] * t->sizes[d]) return false;
+    uint64_t next = 0; // stride * size of the latest dimension with several indexes
+    bool     several = false;
+    for (int d = 1; d < 5; d++)
+    {
+        if (t->sizes[d] <= 1) continue;
+        if (d > 1 && (uint64_t) t->strides[d] != (uint64_t) t->strides[d - 1] * t->sizes[d - 1]) return false;
+        if (several && t->strides[d] != next) return false;
+        next = (uint64_t) t->strides[d] * t->sizes[d];
+        several = true;
+    }
     return true;
 }
 

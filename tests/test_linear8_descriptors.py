@@ -1,4 +1,6 @@
 """Python descriptors of the 8-bit linear layer (no GPU): what the calls are told about a tensor stays inside its buffer."""
+import os
+
 import numpy as np
 import pytest
 
@@ -88,3 +90,25 @@ def test_windows_of_windows():
             t.window(*bad)
     with pytest.raises(ValueError):
         w.window(3, [8, 3])
+
+
+def test_one_pitch_over_a_dimension_of_one_index():
+    """The stride of a dimension of one index says nothing: rows behind it have to follow from the dimension before."""
+    if not os.path.exists(abi.LIB_PATH):
+        pytest.skip("libmme_hip.so has not been built (python -m intel_gaudi3_software_amd.build)")
+    MIB = 1 << 20
+
+    def one_pitch(sizes, strides, out_strides=None):
+        o, x = (abi.make_tensor(at * MIB, sizes, t, 0, 0, None, dim=5) for at, t in ((2048, abi.INT8), (1, abi.BF16)))
+        for t, st in ((x, strides), (o, out_strides or o.strides)):
+            for d in range(5):
+                t.strides[d] = st[d]
+        return abi.plan_quantize_rows(o, 4096 * MIB, x)["one_pitch"]
+
+    assert one_pitch([64, 3, 1, 4, 1], [1, 100, 300, 300, 1200]) == 1
+    assert one_pitch([64, 3, 1, 4, 1], [1, 100, 700, 700, 2800]) == 0   # (planes 700 apart, three rows of pitch 100 in each)
+    assert one_pitch([64, 3, 1, 1, 4], [1, 100, 5, 700, 700]) == 0
+    assert one_pitch([64, 3, 1, 4, 1], [1, 64, 192, 192, 768], [1, 64, 1000, 1000, 4000]) == 0
+    assert one_pitch([64, 1, 1, 5, 1], [1, 100, 100, 100, 500]) == 1
+    assert one_pitch([64, 3, 4, 1, 1], [1, 0, 0, 0, 0]) == 1            # (one row for all)
+    assert one_pitch([64, 3, 1, 4, 1], [1, 0, 100, 100, 400]) == 0      # (one row for the three of a plane)
