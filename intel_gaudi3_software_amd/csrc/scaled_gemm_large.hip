@@ -8,9 +8,9 @@
 // read; one barrier per stage; 16-byte chunks of the 64-byte rows swizzled by (row >> 2) & 3, which keeps the fragment reads free of bank
 // conflicts.  New here: int8 (two 32-k instructions where fp8 has one of 64 k), rows of any count on both sides (the copies of a
 // partial tile read its last row again, its stores are predicated), K of any length from 256 on (what is left behind the last whole
-// stage is multiplied from registers), and an epilogue with a scale per row and per column.  Measured: int8 4096^3 with a bias 63 us
-// (2171 TOP/s), fp8 57 us; fp8, four products of 2048 x 14336 x 4096 421 us (2284 TFLOP/s); 8192 x 4096 x 256, whose time is the
-// stores', 26 us.
+// stage is multiplied from registers), and an epilogue with a scale per row and per column.  Measured: int8 4096^3 with a bias 64 us
+// (2150 TOP/s), fp8 57 us; four products of 2048 x 14336 x 4096 in fp8 425 us (2260 TFLOP/s), in int8 455; 8192 x 4096 x 256, whose time
+// is the stores', 25 us.
 #include "scaled_gemm_common.hpp"
 
 namespace mme
