@@ -177,3 +177,60 @@ def test_convolution_weights_behind_a_dimension_of_one_index(calc, op):
             calc.synchronize()
             outs.append(out)
     assert torch.equal(outs[0], outs[1]) and torch.any(outs[0] != 0)
+
+
+FIRST_CALLS = """
+import torch
+from intel_gaudi3_software_amd import HipCalculator, MmeSimTensor, abi
+g = torch.Generator(device="cuda"); g.manual_seed(1)
+T = lambda x, t, *fp8: MmeSimTensor(list(x.shape)[::-1], x.dim(), t, x, *fp8)
+codes = lambda *s: torch.randint(0, 0x70, s, generator=g, device="cuda", dtype=torch.int32).to(torch.uint8)
+real = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+calls, outs = [], []
+side = torch.cuda.Stream()
+c = HipCalculator()
+c.setStream(side.cuda_stream)
+for t in ((abi.INT8,), (abi.FP8_143, 7, abi.MINIMAL_INF_NAN), (abi.FP8_152, 15)):
+    for M, N, K in ((4, 512, 512), (4, 512, 520), (20, 16384, 512), (70, 4000, 512), (70, 4000, 333), (2001, 2001, 392), (2001, 2001, 385), (4000, 4001, 512)):
+        o = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+        outs.append(o)
+        calls.append(lambda a=(T(o, abi.BF16), T(codes(M, K), *t), None, T(codes(N, K), *t), None): c.scaledGemm(*a))
+for rows, width in ((40, 100), (300, 4096), (300, 14336), (20, 20000)):
+    q, s = torch.zeros(rows, width, dtype=torch.uint8, device="cuda"), torch.zeros(rows, device="cuda")
+    outs += [q, s]
+    calls.append(lambda a=(T(q, abi.INT8), s, T(real(rows, width), abi.BF16), T(real(rows, width), abi.BF16)): c.quantizeRows(*a))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    for f in calls:
+        f()
+torch.cuda.synchronize()
+assert not any(bool(o.any()) for o in outs)
+got = []
+for k in range(3):
+    for o in outs:
+        o.zero_()
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    got.append([o.clone() for o in outs])
+for o in outs:
+    o.zero_()
+torch.cuda.synchronize()
+for f in calls:
+    f()
+c.synchronize()
+for k in range(3):
+    assert all(bool(a.any()) and torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(got[k], outs)), k
+print("the same")
+"""
+
+
+def test_first_calls_of_a_process_are_recorded():
+    """Every form recorded into a graph by a process that has made no call before: nothing is asked of the runtime that a recording refuses."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-u", "-c", FIRST_CALLS], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, timeout=100)
+    assert r.returncode == 0 and b"the same" in r.stdout, r.stdout.decode(errors="replace")[-2000:]
