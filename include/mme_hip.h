@@ -540,10 +540,11 @@ int mme_hip_absmax_dev(mme_hip_handle h, float* out_absmax, const float* in, siz
  * with q the largest value of the output type: 127 (MME_HIP_INT8); 240 2^(7-bias) (fp8_143 in full inf/NaN mode) or 448 2^(7-bias)
  * (minimal mode); 57344 2^(15-bias) (fp8_152 in full mode).  Other inf/NaN modes: EUNSUPPORTED.  No code is an inf or NaN.
  * x and gate: bf16, fp16 (exponent bias 15, full mode) or fp32, the same type and sizes as each other; the sizes of out.
- * row_scales: one float per row, dense in the order of the rows (dimension 1 fastest).  Arithmetic in fp32: what is rounded to a code is
- * within 2^-23 of v_i q / max |v| (a value that close to the middle of two codes may get either), a gate within 2^-21 of its own (the tanh
- * form's exponent has five roundings before that); the scale is rounded once from fp64.  A row of zeros gets the scale 0 and codes of zero.  A row that holds an inf or NaN (or whose gated
- * products overflow fp32) gets the scale NaN and codes 0: NaN reaches every output of its row in the product, and no other.
+ * row_scales: one float per row, dense in the order of the rows (dimension 1 fastest).  Arithmetic in fp32: what is rounded to a
+ * code is within 2^-23 of v_i q / max |v| (a value that close to the middle of two codes may get either), a gate within 2^-21 of
+ * its own (the tanh form's exponent has five roundings before that); the scale is rounded once from fp64.  A row of zeros gets the
+ * scale 0 and codes of zero.  A row that holds an inf or NaN (or whose gated products overflow fp32) gets the scale NaN and codes
+ * 0: NaN reaches every output of its row in the product, and no other.
  * Where the scale itself falls below 2^-126 it has fewer bits, like any denormal.  Up to 2^28 - 16 rows (more: EUNSUPPORTED).
  */
 int mme_hip_quantize_rows_dev(mme_hip_handle        h,
@@ -586,9 +587,9 @@ int mme_hip_rms_norm_quantize_dev(mme_hip_handle        h,
  *     code has all exponent bits set, which holds for what the quantisers write: EUNSUPPORTED without it.
  * The sum is rounded to fp32, multiplied by the scale of x, then by that of w (together with the addition of the bias in one
  * rounding), then rounded to nearest even into out's type; out of range becomes inf.  fp16 outputs have exponent bias 15.
- * The result is the same, bit for bit, for every call with the same operands, sizes and strides, and with the operands' addresses multiples of
- * 16 in both calls or in neither (which kernel runs depends on that, and with it the order of fp8 sums; int8 sums have none).  K = 0 gives the bias.  Up to 65535
- * batch elements, K up to 2^30, N up to 2^27 - 16 (more: EUNSUPPORTED).
+ * The result is the same, bit for bit, for every call with the same operands, sizes and strides, and with the operands' addresses
+ * multiples of 16 in both calls or in neither (which kernel runs depends on that, and with it the order of fp8 sums; int8 sums have
+ * none).  K = 0 gives the bias.  Up to 65535 batch elements, K up to 2^30, N up to 2^27 - 16 (more: EUNSUPPORTED).
  */
 int mme_hip_scaled_gemm_dev(mme_hip_handle        h,
                             const mme_hip_tensor* out,
